@@ -76,6 +76,16 @@ ABI = {
     "execute_adam_amp_step_fused_async": (i, [u, up, up, up, up, up, up, up, up, i, ip, f, f, f, f, f, u]),
     "gm_amp_state_current_set": (i, [u]),
     "gm_amp_state_set_current_set": (i, [u, i]),
+    "gm_command_queue_for_stream": (u, [u, vp]),
+    "gm_allocate_workspace": (u, [u, u]),
+    "execute_dropout": (i, [u, u, u, u, u, i, i, f, u, i]),
+    "gm_rng_state_advance": (i, [u, u, u]),
+    "execute_embedding_lookup": (i, [u, u, u, u, u, i, i, i, i, i, i, f, f, u, i]),
+    "gm_embedding_gradient_workspace": (u, [i, i, i]),
+    "execute_embedding_gradient": (i, [u, u, u, u, u, i, i, i, i, i, i, i, f, i, i, f, u, i, u, u]),
+    "gm_linear_cross_entropy_workspace": (u, [i, i, i, u, i, i, i, i]),
+    "gm_linear_cross_entropy_least_workspace": (u, [i, i, i, u, i, i, i, i]),
+    "execute_linear_cross_entropy": (i, [u, u, u, u, u, u, u, u, u, i, i, i, i, i, i, i, i, i, i, i, f, u, i, u, u]),
     "gm_timer_start": (i, [u]),
     "gm_timer_stop": (f, [u]),
     "gm_fill_normal_f32": (i, [u, u, ctypes.c_size_t, ctypes.c_uint64, f, f]),

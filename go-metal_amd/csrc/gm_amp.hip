@@ -1000,3 +1000,17 @@ try {
 }
 
 }  // extern "C"
+
+bool gm::amp_scale_view(uintptr_t amp_state, Context *ctx, AmpScaleView *view)
+{
+    const AmpState *s = amp_from_handle(amp_state);
+    if (!s || s->ctx != ctx) {
+        set_error("the loss-scale state is not one of this device's");
+        return false;
+    }
+    for (int k = 0; k < 2; k++) {
+        view->scale[k] = &s->d_block->slot[k].scale;
+        view->stamp[k] = &s->d_block->slot[k].stamp;
+    }
+    return true;
+}

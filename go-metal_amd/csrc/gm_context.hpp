@@ -78,6 +78,10 @@ Context *resolve_device(uintptr_t device);
 // thread-local and callers may hop threads between calls).
 bool make_current(Context *ctx);
 
+// The stream a command queue of this context stands for (0: the context's own).  false: not a queue of
+// this context, error recorded.
+bool queue_stream(Context *ctx, uintptr_t command_queue, hipStream_t *stream);
+
 // ---- buffer registry: handle (device address) -> allocation length ----
 // base: the address to hand back to hipFree when it differs from the handle (0: the handle itself)
 void registry_add(uintptr_t buffer, size_t bytes, uintptr_t base = 0);
@@ -95,5 +99,14 @@ void lbfgs_forget_range(uintptr_t begin, size_t bytes);                  // L-BF
 // Resolves this GPU's address of the allocation-free step's descriptor table (a __device__
 // array) once, at context creation, with the device current.  false: error recorded.
 bool noalloc_bind_scratch(Context *ctx);
+
+// Where a loss-scale state keeps its scale on the device: two records that steps write in turn; the one with the
+// larger stamp is the state as of now (equal stamps, both 0: the first), so a kernel can pick it when it runs.
+struct AmpScaleView {
+    const float *scale[2] = {nullptr, nullptr};
+    const unsigned long long *stamp[2] = {nullptr, nullptr};
+};
+// false: not a loss-scale state of this context, error recorded.
+bool amp_scale_view(uintptr_t amp_state, Context *ctx, AmpScaleView *view);
 
 }  // namespace gm

@@ -1,0 +1,732 @@
+// Softmax cross entropy of a linear output layer over a large vocabulary, with its gradients, without the logits.
+//
+//   s = x W^T          loss_i = lse(s_i) - s_i[t_i]          dS = (exp(s - lse) - onehot(t)) c
+//   dX = dS W          dW (+)= dS^T x                        c = gradient scale * loss scale (/ counted tokens)
+//
+// Tokens whose target is the ignored one (or no word of the vocabulary) take no part: the others are packed first,
+// so they cost nothing and whatever stands in them reaches no sum.  Then, for as many tokens at a time as the
+// workspace holds:
+//   logits_kernel   a tile of logits stays in registers: of each token's share of a tile its maximum m and the sum of
+//                   exp(s - m) are kept, the target's logit in fp32, and (gradients wanted) exp(s - m) itself
+//   rows_kernel     one token a workgroup: lse from its tiles' maxima and sums, the loss, and exp(s - m) turned into dS
+//                   (the target's entry as expm1 of its fp32 logit: p - 1 of a certain token keeps its digits)
+//   product_kernel  dX and dW
+// 2 N V D operations each: the product of the logits is made once and not again for the gradients; what it costs is
+// the pass of rows_kernel over the workspace.
+#include "gm_matrix.hpp"
+
+#include "../../include/gometal_hip.h"
+
+#include <cmath>
+
+namespace gm {
+
+// What the kernels of one call find out on the device.
+struct LossHead {
+    int count;                 // tokens that take part
+    float coefficient;         // c above
+};
+
+typedef Shape<256, 256, 2, 4, 2> WideShape;       // products of many tiles: 128 KiB of LDS, one workgroup a CU
+typedef Shape<128, 128, 2, 2, 2> SquareShape;     // fewer tiles than a wide shape needs to fill the chip
+typedef Shape<128, 32, 4, 1, 4> FlatShape;        // up to 32 tokens: the weights' stream is all there is
+enum : int { kWide, kSquare, kFlat };
+constexpr int kShapeP[3] = {256, 128, 128}, kShapeQ[3] = {256, 128, 32}, kShapeSpan[3] = {128, 64, 32};
+
+// exp(s - m) in 16 bits is 32768 times itself in fp16, dS of fp16 operands 16384 times itself: both keep clear of the
+// subnormals (down to 2^-29 and 2^-28), and an entry's rounding is 2^-12 of it.
+constexpr float kExpScale = 32768.0f;
+template <typename T>
+constexpr float kSlopeScale = 1.0f;
+template <>
+constexpr float kSlopeScale<_Float16> = 16384.0f;
+
+__device__ inline int chunk_rows(const LossHead *head, int first, int most)
+{
+    const int left = head->count - first;
+    return left < 0 ? 0 : left < most ? left : most;
+}
+
+// ------------------------------------------------------------------------------------------ tokens that count ----
+constexpr int kScanBlock = 1024;
+
+// Packs the tokens that take part: row_of[r] is the r-th one, place_of[i] where token i went (-1: nowhere).
+__global__ void __launch_bounds__(kScanBlock)
+scan_targets_kernel(const int *targets, int n, int vocab, int ignore, int mean, float gradient_scale, AmpScaleView amp, LossHead *head,
+                    int *row_of, int *place_of, int *row_target)
+{
+    __shared__ int of_wave[kScanBlock / 64 + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int done = 0;
+    for (int base = 0; base < n; base += kScanBlock) {
+        const int i = base + (int)threadIdx.x;
+        const int t = i < n ? targets[i] : ignore;
+        const bool counts = i < n && t != ignore && (unsigned)t < (unsigned)vocab;
+        const unsigned long long votes = __ballot(counts);
+        if (lane == 0) of_wave[wave] = __popcll(votes);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int sum = 0;
+            for (int w = 0; w < kScanBlock / 64; w++) {
+                const int c = of_wave[w];
+                of_wave[w] = sum;
+                sum += c;
+            }
+            of_wave[kScanBlock / 64] = sum;
+        }
+        __syncthreads();
+        const int place = done + of_wave[wave] + __popcll(votes & ((1ull << lane) - 1ull));
+        if (i < n) place_of[i] = counts ? place : -1;
+        if (counts) {
+            row_of[place] = i;
+            row_target[place] = t;
+        }
+        done += of_wave[kScanBlock / 64];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        float scale = gradient_scale;
+        if (amp.scale[0]) scale = scale * *amp.scale[*amp.stamp[1] > *amp.stamp[0] ? 1 : 0];
+        head->count = done;
+        head->coefficient = mean ? scale / (float)(done > 0 ? done : 1) : scale;
+    }
+}
+
+// x as the planes of an operand: h, then what of x is left after h, and so on; each rounded to nearest.
+template <typename T>
+__device__ inline void split_store(float x, T *to, int64_t plane, int planes)
+{
+    for (int k = 0; k < planes; k++) {
+        const T part = from_float<T>(x);
+        to[k * plane] = part;
+        x = x - (float)part;
+    }
+}
+
+// Rows of a matrix as operand rows: `width` elements (a multiple of 64) of each, zeros behind the matrix's own `dim`.
+template <typename I, typename T>
+__device__ inline void pack_row(const I *from, T *to, int dim, int width, int64_t plane, int planes)
+{
+    for (int c = threadIdx.x; c < width; c += blockDim.x) split_store<T>(from && c < dim ? (float)from[c] : 0.0f, to + c, plane, planes);
+}
+
+constexpr int kPackBlock = 256;
+
+// Workgroup i < n: token i's activations to their place, or zeros to its outputs.  The rows behind the last counted
+// token, up to a whole step of k, become zeros.
+template <typename I, typename T>
+__global__ void __launch_bounds__(kPackBlock)
+pack_tokens_kernel(const I *x, int64_t x_stride, int n, int dim, int width, const LossHead *head, const int *place_of, T *packed,
+                   int64_t plane, int planes, float *losses, I *dx, int64_t dx_stride)
+{
+    const int i = blockIdx.x;
+    if (i >= n) {
+        const int r = head->count + (i - n), end = (head->count + kStepK - 1) / kStepK * kStepK;
+        if (r < end) pack_row<I, T>(nullptr, packed + (int64_t)r * width, 0, width, plane, planes);
+        return;
+    }
+    const int place = place_of[i];
+    if (place >= 0) {
+        pack_row<I, T>(x + (int64_t)i * x_stride, packed + (int64_t)place * width, dim, width, plane, planes);
+        return;
+    }
+    if (threadIdx.x == 0) losses[i] = 0.0f;
+    if (dx)
+        for (int c = threadIdx.x; c < dim; c += kPackBlock) dx[(int64_t)i * dx_stride + c] = (I)0.0f;
+}
+
+template <typename I, typename T>
+__global__ void __launch_bounds__(kPackBlock)
+pack_weights_kernel(const I *w, int64_t w_stride, int dim, int width, T *packed, int64_t plane, int planes)
+{
+    pack_row<I, T>(w + (int64_t)blockIdx.x * w_stride, packed + (int64_t)blockIdx.x * width, dim, width, plane, planes);
+}
+
+// --------------------------------------------------------------------------------------------------- logits ----
+enum : int { kKeepNothing, kKeepHalf, kKeepFloat };
+
+struct LogitsArgs {
+    Operand w, x;               // x: the chunk's rows
+    PlanePairs pairs;
+    int steps, first, most, vocab, padded;      // padded: vocab up to a whole step of k
+    const LossHead *head;
+    const int *row_target;      // by packed token
+    float *target_logit;
+    float2 *stats;              // [row of the chunk][group]: maximum, sum of exp(s - maximum)
+    int groups, keep;
+    void *kept;                 // [row of the chunk][padded]
+};
+
+template <typename T, typename S>
+__global__ void __launch_bounds__(S::THREADS)
+logits_kernel(LogitsArgs a)
+{
+    __shared__ __attribute__((aligned(1024))) char tiles[S::LDS];
+    const int rows = chunk_rows(a.head, a.first, a.most);
+    uint32_t tp, tq;
+    if (!tile_of(blockIdx.x, (a.vocab + S::BP - 1) / S::BP, (rows + S::BQ - 1) / S::BQ, 8, tp, tq)) return;
+    a.x.rows = rows;
+    const int p0 = (int)tp * S::BP, q0 = (int)tq * S::BQ;
+    f32x4 acc[S::MP][S::MQ];
+    multiply_tiles<T, S, false, false>(a.w, a.x, a.pairs, p0, q0, a.steps, 0, 0, 0, a.steps * a.pairs.count,
+                                       (uint32_t)(uintptr_t)(GM_LDS char *)tiles, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wp = p0 + wave / S::WQ * (S::BP / S::WP) + (lane >> 4) * 4, wq = q0 + wave % S::WQ * (S::BQ / S::WQ) + (lane & 15);
+    const int group = (p0 + wave / S::WQ * (S::BP / S::WP)) / (S::BP / S::WP);
+#pragma unroll
+    for (int j = 0; j < S::MQ; j++) {
+        const int q = wq + j * 16;
+        const bool there = q < rows;
+        const int target = there ? a.row_target[a.first + q] : -1;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < S::MP; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int p = wp + i * 16 + r;
+                if (p >= a.vocab) acc[i][j][r] = -INFINITY;
+                top = fmaxf(top, acc[i][j][r]);
+                if (p == target) a.target_logit[a.first + q] = acc[i][j][r];
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float ref = top == -INFINITY ? 0.0f : top;      // (a share that lies behind the vocabulary: all zeros)
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::MP; i++) {
+            f32x4 e;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                e[r] = a.keep == kKeepFloat ? expf(acc[i][j][r] - ref) : __expf(acc[i][j][r] - ref);
+                sum += e[r];
+            }
+            const int p = wp + i * 16;
+            if (a.keep == kKeepNothing || !there || p >= a.padded) continue;
+            const int64_t at = (int64_t)q * a.padded + p;
+            if (a.keep == kKeepFloat) {
+                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.kept) + at) = e;
+            } else {
+                typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+                f16x4 h;
+#pragma unroll
+                for (int r = 0; r < 4; r++) h[r] = (_Float16)(e[r] * kExpScale);
+                *reinterpret_cast<f16x4 *>(static_cast<_Float16 *>(a.kept) + at) = h;
+            }
+        }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (there && lane < 16) a.stats[(int64_t)q * a.groups + group] = float2{top, sum};
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------- rows ----
+constexpr int kRowBlock = 512;
+
+struct RowsArgs {
+    int first, most, vocab, padded, groups, span;       // span: words of a group
+    const LossHead *head;
+    const int *row_of, *row_target;
+    const float *target_logit;
+    const float2 *stats;
+    float *losses;
+    int keep, planes;
+    void *kept, *slopes;       // kKeepHalf: the same memory
+    int64_t plane;
+};
+
+__device__ inline float block_reduce(float x, bool maximum, float *scratch)
+{
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const float y = __shfl_xor(x, o);
+        x = maximum ? fmaxf(x, y) : x + y;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = scratch[0];
+#pragma unroll
+    for (int w = 1; w < kRowBlock / 64; w++) x = maximum ? fmaxf(x, scratch[w]) : x + scratch[w];
+    return x;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowBlock)
+rows_kernel(RowsArgs a)
+{
+    __shared__ float scratch[kRowBlock / 64];
+    const int rows = chunk_rows(a.head, a.first, a.most), r = blockIdx.x;
+    T *slopes = static_cast<T *>(a.slopes) + (int64_t)r * a.padded;
+    const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (r >= rows) {
+        if (a.keep != kKeepNothing && r < (rows + kStepK - 1) / kStepK * kStepK)      // a whole step of k for dW
+            for (int k = 0; k < a.planes; k++)
+                for (int c = threadIdx.x * 8; c < a.padded; c += kRowBlock * 8) store8(slopes + k * a.plane + c, true, 8, zero);
+        return;
+    }
+    const float2 *stats = a.stats + (int64_t)r * a.groups;
+    float top = -INFINITY;
+    for (int g = threadIdx.x; g < a.groups; g += kRowBlock) top = fmaxf(top, stats[g].x);
+    top = block_reduce(top, true, scratch);
+    float sum = 0.0f;
+    for (int g = threadIdx.x; g < a.groups; g += kRowBlock) sum += stats[g].y * expf(stats[g].x - top);
+    sum = block_reduce(sum, false, scratch);
+    const float lse = top + logf(sum), target_logit = a.target_logit[a.first + r];
+    if (threadIdx.x == 0) a.losses[a.row_of[a.first + r]] = lse - target_logit;
+    if (a.keep == kKeepNothing) return;
+    const int target = a.row_target[a.first + r];
+    const float at_target = expm1f(target_logit - lse);
+    for (int c = threadIdx.x * 8; c < a.padded; c += kRowBlock * 8) {
+        float v[8];
+        float f = c < a.vocab ? expf(stats[c / a.span].x - lse) : 0.0f;
+        if (a.keep == kKeepHalf) {
+            load8(static_cast<const _Float16 *>(a.kept) + (int64_t)r * a.padded + c, true, 8, v);
+            f = f * (1.0f / kExpScale);
+        } else {
+            load8(static_cast<const float *>(a.kept) + (int64_t)r * a.padded + c, true, 8, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = c + e < a.vocab ? (c + e == target ? at_target : v[e] * f) * kSlopeScale<T> : 0.0f;
+        for (int k = 0; k < a.planes; k++) {
+            store8(slopes + k * a.plane + c, true, 8, v);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = v[e] - (float)from_float<T>(v[e]);
+        }
+    }
+}
+
+// The sum (or mean) of the losses and the number of tokens that count; one workgroup, sums in 64 bits in a fixed order.
+__global__ void __launch_bounds__(1024)
+total_kernel(const float *losses, int n, int mean, const LossHead *head, float *loss)
+{
+    __shared__ double part[1024];
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < n; i += 1024) sum += (double)losses[i];
+    part[threadIdx.x] = sum;
+    for (int o = 512; o; o >>= 1) {
+        __syncthreads();
+        if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
+    }
+    if (threadIdx.x == 0) {
+        const int count = head->count;
+        loss[0] = (float)(mean ? part[0] / (double)(count > 0 ? count : 1) : part[0]);
+        loss[1] = (float)count;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- products ----
+struct ProductArgs {
+    Operand p, q;
+    PlanePairs pairs;
+    int first, most;                 // the chunk's tokens
+    int steps;                       // steps of 64 k of one pair; 0: as many as the chunk has tokens (dW)
+    int limit_p;                     // across: the k that exist
+    int splits;                      // parts of the sum; more than one: `partial` takes them
+    float *partial;                  // [split][most][p rows]
+    const LossHead *head;
+    const int *row_of;               // dX: where a packed row belongs
+    float unscale;                   // undoes kSlopeScale
+    void *out;
+    int64_t out_stride;
+    int out_type;
+    int accumulate;                  // add what `out` holds
+    const float *add;                // and this, of out's shape without gaps (nullptr: nothing)
+    bool out_aligned;                // rows of out begin at multiples of four elements
+    bool skip_empty;                 // a chunk without tokens leaves `out` alone
+};
+
+template <typename O>
+__device__ inline void finish4(const ProductArgs &a, O *out, int64_t row, int p, f32x4 v)
+{
+    typedef O Vec __attribute__((ext_vector_type(4)));
+    const int count = a.p.rows - p < 4 ? a.p.rows - p : 4;
+    O *at = out + row * a.out_stride + p;
+    if (a.out_aligned && count == 4) {
+        Vec o;
+        if (a.accumulate) {
+            o = *reinterpret_cast<const Vec *>(at);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (float)o[e] + v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = from_float<O>(v[e]);
+        *reinterpret_cast<Vec *>(at) = o;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < count) at[e] = from_float<O>(a.accumulate ? (float)at[e] + v[e] : v[e]);
+}
+
+// Four outputs of one row: times c, added to what is there, rounded once.
+__device__ inline void finish(const ProductArgs &a, float by, int q, int p, f32x4 v)
+{
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = v[e] * by;
+    if (a.add)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = p + e < a.p.rows ? a.add[(int64_t)q * a.p.rows + p + e] + v[e] : 0.0f;
+    const int64_t row = a.row_of ? a.row_of[a.first + q] : q;
+    if (a.out_type == kFloat32) finish4(a, static_cast<float *>(a.out), row, p, v);
+    else if (a.out_type == kFloat16) finish4(a, static_cast<_Float16 *>(a.out), row, p, v);
+    else finish4(a, static_cast<__bf16 *>(a.out), row, p, v);
+}
+
+// DW: Q is dS across and the sum runs over the chunk's tokens; otherwise dX, Q is dS along.  P lies across in both.
+template <typename T, typename S, bool DW>
+__global__ void __launch_bounds__(S::THREADS)
+product_kernel(ProductArgs a)
+{
+    __shared__ __attribute__((aligned(1024))) char tiles[S::LDS];
+    const int rows = chunk_rows(a.head, a.first, a.most);
+    if (rows == 0 && (!DW || a.skip_empty)) return;
+    if (DW) a.steps = (rows + kStepK - 1) / kStepK;
+    else a.q.rows = rows;
+    const uint32_t tiles_p = (a.p.rows + S::BP - 1) / S::BP, tiles_q = (a.q.rows + S::BQ - 1) / S::BQ;
+    uint32_t tp, tq;
+    if (!tile_of(blockIdx.x, tiles_p, tiles_q, 8, tp, tq)) return;
+    const int limit = DW ? a.steps * kStepK : a.limit_p;
+    const int total = a.steps * a.pairs.count, split = blockIdx.y;
+    const int begin = (int)((int64_t)total * split / a.splits), end = (int)((int64_t)total * (split + 1) / a.splits);
+    const int p0 = (int)tp * S::BP, q0 = (int)tq * S::BQ;
+    f32x4 acc[S::MP][S::MQ];
+    if (begin < end) {
+        multiply_tiles<T, S, true, DW>(a.p, a.q, a.pairs, p0, q0, a.steps, limit, limit, begin, end,
+                                       (uint32_t)(uintptr_t)(GM_LDS char *)tiles, acc);
+    } else {
+#pragma unroll
+        for (int i = 0; i < S::MP; i++)
+#pragma unroll
+            for (int j = 0; j < S::MQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const float by = a.head->coefficient * a.unscale;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wp = p0 + wave / S::WQ * (S::BP / S::WP) + (lane >> 4) * 4, wq = q0 + wave % S::WQ * (S::BQ / S::WQ) + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < S::MQ; j++) {
+        const int q = wq + j * 16;
+        if (q >= a.q.rows) continue;
+#pragma unroll
+        for (int i = 0; i < S::MP; i++) {
+            const int p = wp + i * 16;
+            if (p >= a.p.rows) continue;
+            if (a.splits > 1) {
+                float *at = a.partial + ((int64_t)split * a.most + q) * a.p.rows + p;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (p + e < a.p.rows) at[e] = acc[i][j][e];
+            } else {
+                finish(a, by, q, p, acc[i][j]);
+            }
+        }
+    }
+}
+
+// The parts of a split sum, added up in order; four outputs a lane.
+__global__ void __launch_bounds__(256)
+join_splits_kernel(ProductArgs a)
+{
+    const int rows = chunk_rows(a.head, a.first, a.most);
+    const int per_row = (a.p.rows + 3) / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int q = (int)(i / per_row), p = (int)(i - (int64_t)q * per_row) * 4;
+    if (q >= rows) return;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; s++) {
+        const float *at = a.partial + ((int64_t)s * a.most + q) * a.p.rows + p;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += p + e < a.p.rows ? at[e] : 0.0f;
+    }
+    finish(a, a.head->coefficient * a.unscale, q, p, v);
+}
+
+// ------------------------------------------------------------------------------------------------ host side ----
+// Everything that follows from the sizes: what lies where in the workspace, and which shape each product takes.
+struct LossPlan {
+    int n, vocab, dim, width, padded, chunk, chunks;
+    int operand_type;                      // kFloat16 or kBFloat16
+    int planes, slope_planes, keep;        // planes of x (and W); of dS
+    bool gradients, pack_weights, sum_weights;      // sum_weights: dW of several chunks in 16 bits needs fp32 sums
+    int logits_shape, groups, dx_shape, dx_splits, dw_shape;
+    size_t head, row_of, place_of, row_target, target_logit, x, w, stats, kept, slopes, partial, sums, bytes;
+};
+
+constexpr int kLeastChunk = 256;
+constexpr size_t kKeptBytes = (size_t)4 << 30;      // of exp(s - m) and dS together, unless one chunk needs more
+
+static int shape_for(int64_t p, int64_t q)
+{
+    if (q <= kShapeQ[kFlat]) return kFlat;
+    // a wide tile needs a CU to itself: with fewer of them than CUs the smaller ones are spread better
+    return ((p + 255) / 256) * ((q + 255) / 256) >= 256 ? kWide : kSquare;
+}
+
+static int tiles(int shape, int64_t p, int64_t q)
+{
+    return (int)(((p + kShapeP[shape] - 1) / kShapeP[shape]) * ((q + kShapeQ[shape] - 1) / kShapeQ[shape]));
+}
+
+static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_type, int gradient_type, bool gradients, int chunk)
+{
+    const auto up = [](size_t v, size_t to) { return (v + to - 1) / to * to; };
+    LossPlan s{};
+    s.n = n, s.vocab = vocab, s.dim = dim, s.gradients = gradients;
+    s.width = (int)up((size_t)dim, kStepK), s.padded = (int)up((size_t)vocab, kStepK);
+    s.operand_type = data_type == kFloat32 ? kBFloat16 : data_type;
+    s.planes = data_type == kFloat32 ? 3 : 1;
+    s.slope_planes = data_type == kFloat32 ? 3 : gradient_type == kFloat32 ? 2 : 1;
+    s.keep = !gradients ? kKeepNothing : s.slope_planes == 1 ? kKeepHalf : kKeepFloat;
+    s.pack_weights = data_type == kFloat32 || !weights_fit;
+    const size_t entry = s.keep == kKeepNothing ? 0 : s.keep == kKeepHalf ? 2 : 4 + 2 * s.slope_planes;
+    if (chunk <= 0) {
+        size_t most = entry ? kKeptBytes / (entry * s.padded) / kLeastChunk * kLeastChunk : (size_t)n;
+        if (most < kLeastChunk) most = kLeastChunk;
+        chunk = most < (size_t)n ? (int)most : n;
+    }
+    s.chunk = chunk < n ? chunk : (n > 0 ? n : 1);
+    s.chunks = n > 0 ? (n + s.chunk - 1) / s.chunk : 1;
+    s.sum_weights = gradients && s.chunks > 1 && gradient_type != kFloat32;
+    s.logits_shape = shape_for(vocab, s.chunk);
+    s.groups = (vocab + kShapeP[s.logits_shape] - 1) / kShapeP[s.logits_shape] * (kShapeP[s.logits_shape] / kShapeSpan[s.logits_shape]);
+    if (gradients) {
+        s.dx_shape = shape_for(dim, s.chunk);
+        // few outputs, a long sum: parts of it until every CU has work (two workgroups of the smaller shapes fit a CU)
+        const int tile = tiles(s.dx_shape, dim, s.chunk), want = s.dx_shape == kWide ? 256 : 512, steps = s.padded / kStepK;
+        s.dx_splits = tile >= want ? 1 : want / tile < steps / 8 ? want / tile : steps / 8;
+        if (s.dx_splits < 1) s.dx_splits = 1;
+        s.dw_shape = shape_for(dim, vocab);
+        if (s.dw_shape == kFlat) s.dw_shape = kSquare;
+    }
+    const size_t rows = up((size_t)n, kStepK), chunk_rows = up((size_t)s.chunk, kStepK);
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += up(bytes, 1024);
+        return here;
+    };
+    s.head = take(sizeof(LossHead));
+    s.row_of = take(4 * rows), s.place_of = take(4 * rows), s.row_target = take(4 * rows), s.target_logit = take(4 * rows);
+    s.x = take(rows * s.width * 2 * s.planes);
+    s.w = take(s.pack_weights ? (size_t)vocab * s.width * 2 * s.planes : 0);
+    s.stats = take(sizeof(float2) * (size_t)s.chunk * s.groups);
+    s.kept = take(s.keep == kKeepNothing ? 0 : chunk_rows * s.padded * (s.keep == kKeepHalf ? 2 : 4));
+    s.slopes = s.keep == kKeepFloat ? take(chunk_rows * s.padded * 2 * s.slope_planes) : s.kept;
+    s.partial = take(gradients && s.dx_splits > 1 ? (size_t)s.dx_splits * s.chunk * dim * 4 : 0);
+    s.sums = take(s.sum_weights ? (size_t)vocab * dim * 4 : 0);
+    s.bytes = at;
+    return s;
+}
+
+// The largest chunk whose plan fits the workspace; bytes of the smallest possible one otherwise.
+static bool fitting_plan(LossPlan &s, size_t bytes, int n, int vocab, int dim, bool weights_fit, int data_type, int gradient_type,
+                         bool gradients)
+{
+    s = loss_plan(n, vocab, dim, weights_fit, data_type, gradient_type, gradients, 0);
+    while (s.bytes > bytes && s.chunk > kLeastChunk) {
+        const int half = (s.chunk / 2 + kLeastChunk - 1) / kLeastChunk * kLeastChunk;
+        s = loss_plan(n, vocab, dim, weights_fit, data_type, gradient_type, gradients, half < s.chunk ? half : kLeastChunk);
+    }
+    return s.bytes <= bytes;
+}
+
+static bool weights_fit(uintptr_t weight, int dim, int stride, int data_type)
+{
+    return data_type != kFloat32 && weight != 0 && weight % 16 == 0 && dim % kStepK == 0 && stride % 8 == 0;
+}
+
+static constexpr PlanePairs kOnePair = {1, 0x0};
+// fp32 by three planes of eight bits: the six products of 2^-16 and more, the small ones first
+// (codes: P plane + 4 Q plane)
+static constexpr PlanePairs kSixPairs = {6, 0x041528};
+// x (one plane) with dS (two): the rest first
+static constexpr PlanePairs kSlopePairs = {2, 0x04};
+
+struct LossCall {
+    uintptr_t hidden, weight, targets, losses, loss, dx, dw;
+    int hidden_stride, weight_stride, dx_stride, dw_stride, data_type, gradient_type, ignore, mean, accumulate;
+    float gradient_scale;
+    AmpScaleView amp;
+    char *space;
+};
+
+template <typename T>
+static void launch_logits(int shape, const LogitsArgs &a, int rows, hipStream_t stream)
+{
+    const int grid = (tiles(shape, a.vocab, rows) + 7) / 8 * 8;
+    if (shape == kWide) logits_kernel<T, WideShape><<<grid, WideShape::THREADS, 0, stream>>>(a);
+    else if (shape == kSquare) logits_kernel<T, SquareShape><<<grid, SquareShape::THREADS, 0, stream>>>(a);
+    else logits_kernel<T, FlatShape><<<grid, FlatShape::THREADS, 0, stream>>>(a);
+}
+
+template <typename T, bool DW>
+static void launch_product(int shape, const ProductArgs &a, int p, int q, hipStream_t stream)
+{
+    const dim3 grid((tiles(shape, p, q) + 7) / 8 * 8, a.splits);
+    if (shape == kWide) product_kernel<T, WideShape, DW><<<grid, WideShape::THREADS, 0, stream>>>(a);
+    else if (shape == kSquare) product_kernel<T, SquareShape, DW><<<grid, SquareShape::THREADS, 0, stream>>>(a);
+    else if constexpr (!DW) product_kernel<T, FlatShape, DW><<<grid, FlatShape::THREADS, 0, stream>>>(a);
+}
+
+// I: what the caller's tensors hold; T: what the matrix cores take.
+template <typename I, typename T>
+static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream)
+{
+    char *space = c.space;
+    LossHead *head = reinterpret_cast<LossHead *>(space + s.head);
+    int *row_of = reinterpret_cast<int *>(space + s.row_of), *place_of = reinterpret_cast<int *>(space + s.place_of);
+    int *row_target = reinterpret_cast<int *>(space + s.row_target);
+    float *target_logit = reinterpret_cast<float *>(space + s.target_logit);
+    T *x = reinterpret_cast<T *>(space + s.x);
+    float *losses = reinterpret_cast<float *>(c.losses);
+    const size_t rows = ((size_t)s.n + kStepK - 1) / kStepK * kStepK, chunk_rows = ((size_t)s.chunk + kStepK - 1) / kStepK * kStepK;
+    const int64_t x_plane = (int64_t)rows * s.width, w_plane = (int64_t)s.vocab * s.width, slope_plane = (int64_t)chunk_rows * s.padded;
+
+    scan_targets_kernel<<<1, kScanBlock, 0, stream>>>(reinterpret_cast<const int *>(c.targets), s.n, s.vocab, c.ignore, c.mean,
+                                                      c.gradient_scale, c.amp, head, row_of, place_of, row_target);
+    pack_tokens_kernel<I, T><<<s.n + kStepK, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.hidden), c.hidden_stride, s.n, s.dim,
+                                                                      s.width, head, place_of, x, x_plane, s.planes, losses,
+                                                                      reinterpret_cast<I *>(c.dx), c.dx_stride);
+    Operand w{reinterpret_cast<const short *>(c.weight), c.weight_stride, 0, s.vocab};
+    if (s.pack_weights) {
+        pack_weights_kernel<I, T><<<s.vocab, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight), c.weight_stride, s.dim, s.width,
+                                                                      reinterpret_cast<T *>(space + s.w), w_plane, s.planes);
+        w = Operand{reinterpret_cast<const short *>(space + s.w), s.width, w_plane, s.vocab};
+    }
+    const PlanePairs pairs = s.planes == 3 ? kSixPairs : kOnePair;
+    for (int k = 0; k < s.chunks; k++) {
+        const int first = k * s.chunk, most = s.n - first < s.chunk ? s.n - first : s.chunk;
+        if (most <= 0 && k > 0) break;
+        const Operand xs{reinterpret_cast<const short *>(x + (int64_t)first * s.width), s.width, x_plane, 0};
+        const int tokens = most > 0 ? most : 0;
+        LogitsArgs l{w, xs, pairs, s.width / kStepK, first, tokens, s.vocab, s.padded, head, row_target, target_logit,
+                     reinterpret_cast<float2 *>(space + s.stats), s.groups, s.keep, space + s.kept};
+        RowsArgs r{first, tokens, s.vocab, s.padded, s.groups, kShapeSpan[s.logits_shape], head, row_of, row_target, target_logit,
+                   reinterpret_cast<const float2 *>(space + s.stats), losses, s.keep, s.slope_planes, space + s.kept, space + s.slopes,
+                   slope_plane};
+        if (tokens > 0) {
+            launch_logits<T>(s.logits_shape, l, tokens, stream);
+            rows_kernel<T><<<(tokens + kStepK - 1) / kStepK * kStepK, kRowBlock, 0, stream>>>(r);
+        }
+        if (!s.gradients) continue;
+        const Operand slopes{reinterpret_cast<const short *>(space + s.slopes), s.padded, slope_plane, 0};
+        if (c.dx && tokens > 0) {
+            ProductArgs a{};
+            a.p = w, a.p.rows = s.dim, a.q = slopes, a.pairs = pairs;
+            a.first = first, a.most = tokens, a.steps = s.padded / kStepK, a.limit_p = s.vocab;
+            a.splits = s.dx_splits, a.partial = reinterpret_cast<float *>(space + s.partial);
+            a.head = head, a.row_of = row_of, a.unscale = 1.0f / kSlopeScale<T>;
+            a.out = reinterpret_cast<void *>(c.dx), a.out_stride = c.dx_stride, a.out_type = c.data_type;
+            a.out_aligned = c.dx % (4 * sizeof(I)) == 0 && c.dx_stride % 4 == 0;
+            launch_product<T, false>(s.dx_shape, a, s.dim, tokens, stream);
+            if (s.dx_splits > 1)
+                join_splits_kernel<<<(unsigned)(((int64_t)tokens * ((s.dim + 3) / 4) + 255) / 256), 256, 0, stream>>>(a);
+        }
+        if (c.dw) {
+            ProductArgs a{};
+            a.p = xs, a.p.rows = s.dim, a.q = slopes, a.q.rows = s.vocab;
+            a.pairs = s.planes == 3 ? kSixPairs : s.slope_planes == 2 ? kSlopePairs : kOnePair;
+            a.first = first, a.most = tokens, a.splits = 1, a.head = head, a.unscale = 1.0f / kSlopeScale<T>;
+            const bool last = k + 1 == s.chunks;
+            float *sums = reinterpret_cast<float *>(space + s.sums);
+            if (s.sum_weights && !last) {
+                a.out = sums, a.out_stride = s.dim, a.out_type = kFloat32, a.accumulate = k > 0;
+                a.out_aligned = s.dim % 4 == 0;
+            } else {
+                a.out = reinterpret_cast<void *>(c.dw), a.out_stride = c.dw_stride, a.out_type = c.gradient_type;
+                a.out_aligned = c.dw % (4 * type_bytes(c.gradient_type)) == 0 && c.dw_stride % 4 == 0;
+                a.accumulate = c.accumulate || (k > 0 && !s.sum_weights);
+                a.add = s.sum_weights && k > 0 ? sums : nullptr;
+            }
+            a.skip_empty = a.accumulate && !a.add;
+            launch_product<T, true>(s.dw_shape, a, s.dim, s.vocab, stream);
+        }
+    }
+    total_kernel<<<1, 1024, 0, stream>>>(losses, s.n, c.mean, head, reinterpret_cast<float *>(c.loss));
+}
+
+static bool loss_sizes(int n, int vocab, int dim, int data_type, int gradient_type)
+{
+    return n >= 0 && n <= 1 << 24 && vocab > 0 && vocab <= 1 << 24 && dim > 0 && dim <= 1 << 20 && known_type(data_type) &&
+           (gradient_type == kFloat32 || gradient_type == data_type);
+}
+
+}  // namespace gm
+
+using namespace gm;
+
+extern "C" {
+
+uintptr_t gm_linear_cross_entropy_workspace(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer, int weight_stride,
+                                            int data_type, int gradient_type, int with_gradients)
+{
+    if (!loss_sizes(num_tokens, vocab_size, dim, data_type, gradient_type)) return 0;
+    return loss_plan(num_tokens, vocab_size, dim, weights_fit(weight_buffer, dim, weight_stride, data_type), data_type, gradient_type,
+                     with_gradients != 0, 0).bytes;
+}
+
+uintptr_t gm_linear_cross_entropy_least_workspace(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer, int weight_stride,
+                                                  int data_type, int gradient_type, int with_gradients)
+{
+    if (!loss_sizes(num_tokens, vocab_size, dim, data_type, gradient_type)) return 0;
+    LossPlan s;
+    fitting_plan(s, 0, num_tokens, vocab_size, dim, weights_fit(weight_buffer, dim, weight_stride, data_type), data_type, gradient_type,
+                 with_gradients != 0);
+    return s.bytes;
+}
+
+int execute_linear_cross_entropy(uintptr_t device, uintptr_t command_queue, uintptr_t hidden_buffer, uintptr_t weight_buffer,
+                                 uintptr_t target_buffer, uintptr_t losses_buffer, uintptr_t loss_buffer,
+                                 uintptr_t hidden_gradient_buffer, uintptr_t weight_gradient_buffer, int num_tokens, int vocab_size,
+                                 int dim, int hidden_stride, int weight_stride, int hidden_gradient_stride, int weight_gradient_stride,
+                                 int data_type, int gradient_type, int ignore_index, int mean, float gradient_scale, uintptr_t amp_state,
+                                 int accumulate, uintptr_t workspace, uintptr_t workspace_bytes)
+try {
+    clear_error();
+    if (device == 0) return kRcDevice;
+    if (hidden_buffer == 0 || weight_buffer == 0 || target_buffer == 0 || losses_buffer == 0 || loss_buffer == 0) return kRcNil;
+    if (!known_type(data_type) || (gradient_type != kFloat32 && gradient_type != data_type)) return kRcType;
+    const bool gradients = hidden_gradient_buffer != 0 || weight_gradient_buffer != 0;
+    if (!loss_sizes(num_tokens, vocab_size, dim, data_type, gradient_type) || hidden_stride < dim || weight_stride < dim ||
+        (hidden_gradient_buffer != 0 && hidden_gradient_stride < dim) || (weight_gradient_buffer != 0 && weight_gradient_stride < dim)) {
+        set_error("sizes: %d tokens, vocabulary %d, dimension %d, strides %d, %d, %d and %d", num_tokens, vocab_size, dim, hidden_stride,
+                  weight_stride, hidden_gradient_stride, weight_gradient_stride);
+        return kRcRange;
+    }
+    const size_t in = type_bytes(data_type), out = type_bytes(gradient_type), n = (size_t)num_tokens, v = (size_t)vocab_size, d = (size_t)dim;
+    if (!element_aligned("hidden", hidden_buffer, in) || !element_aligned("weight", weight_buffer, in) ||
+        !element_aligned("targets", target_buffer, 4) || !element_aligned("losses", losses_buffer, 4) ||
+        !element_aligned("loss", loss_buffer, 4) || !element_aligned("hidden gradient", hidden_gradient_buffer, in) ||
+        !element_aligned("weight gradient", weight_gradient_buffer, out) ||
+        !rows_fit("hidden", hidden_buffer, n, d, (size_t)hidden_stride, in) ||
+        !rows_fit("weight", weight_buffer, v, d, (size_t)weight_stride, in) || !rows_fit("targets", target_buffer, 1, n, n, 4) ||
+        !rows_fit("losses", losses_buffer, 1, n, n, 4) || !rows_fit("loss", loss_buffer, 1, 2, 2, 4) ||
+        (hidden_gradient_buffer && !rows_fit("hidden gradient", hidden_gradient_buffer, n, d, (size_t)hidden_gradient_stride, in)) ||
+        (weight_gradient_buffer && !rows_fit("weight gradient", weight_gradient_buffer, v, d, (size_t)weight_gradient_stride, out)))
+        return kRcRange;
+    LossPlan plan;
+    if (!fitting_plan(plan, workspace ? (size_t)workspace_bytes : 0, num_tokens, vocab_size, dim,
+                      weights_fit(weight_buffer, dim, weight_stride, data_type), data_type, gradient_type, gradients) ||
+        workspace % 1024 != 0 || !rows_fit("workspace", workspace, 1, plan.bytes, plan.bytes, 1)) {
+        set_error("the workspace holds %zu bytes (or is not aligned to 1024): at least %zu are needed", (size_t)workspace_bytes, plan.bytes);
+        return kRcWorkspace;
+    }
+    Context *ctx = resolve_device(device);
+    if (!ctx) return kRcNoGpu;
+    hipStream_t stream;
+    if (!queue_stream(ctx, command_queue, &stream)) return kRcQueue;
+    LossCall c{hidden_buffer, weight_buffer, target_buffer, losses_buffer, loss_buffer, hidden_gradient_buffer, weight_gradient_buffer,
+               hidden_stride, weight_stride, hidden_gradient_stride, weight_gradient_stride, data_type, gradient_type, ignore_index,
+               mean != 0, accumulate != 0, gradient_scale, AmpScaleView{}, reinterpret_cast<char *>(workspace)};
+    if (amp_state != 0 && !amp_scale_view(amp_state, ctx, &c.amp)) return kRcAmp;
+    DeviceScope scope(ctx);
+    if (!scope.ok()) return kRcHip;
+    if (data_type == kFloat32) launch_loss<float, __bf16>(c, plan, stream);
+    else if (data_type == kFloat16) launch_loss<_Float16, _Float16>(c, plan, stream);
+    else launch_loss<__bf16, __bf16>(c, plan, stream);
+    return hip_ok(hipGetLastError(), "linear cross entropy launch") ? 0 : kRcHip;
+} catch (...) {
+    note_exception();
+    return kRcHip;
+}
+
+}  // extern "C"

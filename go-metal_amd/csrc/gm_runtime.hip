@@ -404,6 +404,7 @@ void destroy_metal_device(uintptr_t device)
 struct CommandQueue {
     uint64_t magic;
     Context *ctx;
+    hipStream_t stream;      // the context's, or the caller's (gm_command_queue_for_stream)
 };
 static const uint64_t kQueueMagic = 0x676D5F7175657565ull;   // "gm_queue"
 
@@ -412,7 +413,19 @@ try {
     if (device == 0) return 0;
     Context *ctx = resolve_device(device);
     if (!ctx) return 0;
-    return reinterpret_cast<uintptr_t>(new CommandQueue{kQueueMagic, ctx});
+    return reinterpret_cast<uintptr_t>(new CommandQueue{kQueueMagic, ctx, ctx->stream});
+} catch (...) {
+    note_exception();
+    return 0;
+}
+
+uintptr_t gm_command_queue_for_stream(uintptr_t device, void *hip_stream)
+try {
+    clear_error();
+    if (device == 0) return 0;
+    Context *ctx = resolve_device(device);
+    if (!ctx) return 0;
+    return reinterpret_cast<uintptr_t>(new CommandQueue{kQueueMagic, ctx, reinterpret_cast<hipStream_t>(hip_stream)});
 } catch (...) {
     note_exception();
     return 0;
@@ -436,6 +449,22 @@ try {
     const size_t aligned = ((size_t)size + 15) / 16 * 16;
     void *p = nullptr;
     if (!hip_ok(hipMalloc(&p, aligned), "hipMalloc")) return 0;
+    registry_add(reinterpret_cast<uintptr_t>(p), aligned);
+    return reinterpret_cast<uintptr_t>(p);
+} catch (...) {
+    note_exception();
+    return 0;
+}
+
+uintptr_t gm_allocate_workspace(uintptr_t device, uintptr_t bytes)
+try {
+    clear_error();
+    if (device == 0 || bytes == 0 || bytes > (uintptr_t)1 << 46) return 0;
+    Context *ctx = resolve_device(device);
+    if (!ctx || !make_current(ctx)) return 0;
+    const size_t aligned = (bytes + 255) / 256 * 256;
+    void *p = nullptr;
+    if (!hip_ok(hipMalloc(&p, aligned), "hipMalloc(workspace)")) return 0;
     registry_add(reinterpret_cast<uintptr_t>(p), aligned);
     return reinterpret_cast<uintptr_t>(p);
 } catch (...) {
@@ -806,3 +835,16 @@ try {
 }
 
 }  // extern "C"
+
+bool gm::queue_stream(Context *ctx, uintptr_t command_queue, hipStream_t *stream)
+{
+    *stream = ctx->stream;
+    if (command_queue == 0) return true;
+    const auto *q = reinterpret_cast<const CommandQueue *>(command_queue);
+    if (q->magic != kQueueMagic || q->ctx != ctx) {
+        set_error("the command queue is not one of this device's");
+        return false;
+    }
+    *stream = q->stream;
+    return true;
+}

@@ -390,6 +390,106 @@ int gm_lbfgs_dot(uintptr_t device, uintptr_t *a_buffers, uintptr_t *b_buffers, i
 int gm_plan_cache_stats(uintptr_t device, uint64_t *plan_builds, uint64_t *table_allocations,
                         int *cached_plans);
 
+/* ------------------------------------------------------------------------ */
+/* The two ends of a language model's training step (additions).              */
+/* What comes before an optimizer step: rows of the token table on the way    */
+/* in, the loss on the way out, and the gradients that the step takes.        */
+/*                                                                            */
+/* Types: Float32 = 0, Float16 = 2 (memory/tensor.go:12-17), BFloat16 = 4.    */
+/* Strides are elements from row to row (at least the row's length).  Any     */
+/* alignment an element may have is accepted; rows that begin at multiples of */
+/* 16 bytes are faster.                                                       */
+/* command_queue: 0 for the library's stream, or a queue: of                  */
+/* create_command_queue (the library's stream too) or                         */
+/* gm_command_queue_for_stream.  Every call enqueues and returns; none of     */
+/* them allocates, copies or waits, so they may be captured into a HIP graph. */
+/* Two calls that may run at once need a workspace each, and so do two        */
+/* captured graphs.  Results repeat bit for bit: no sum depends on the order  */
+/* in which workgroups finish.                                                */
+/* Codes: -1 device 0; -2 not a queue of this device; -3 no GPU; -4 a needed  */
+/* handle is 0; -5 a size, stride, alignment or probability out of range, or  */
+/* a buffer of this library that is too short; -6 HIP error; -16 not a        */
+/* loss-scale state; -18 the workspace is too small (gm_last_error says how   */
+/* much is needed); -19 a type, or a pair of types, that is not offered.      */
+/* Nothing is launched on any of them but -6.                                 */
+/* ------------------------------------------------------------------------ */
+
+/* A queue for work on a caller's own HIP stream (NULL: the legacy default stream): the operators below then run
+ * there, ordered with the caller's work without events.  Released with release_command_queue, which does not touch
+ * the stream.  0: device 0 or no GPU.  The optimizer steps stay on the library's stream: order them with
+ * gm_wait_for_stream / gm_signal_stream. */
+uintptr_t gm_command_queue_for_stream(uintptr_t device, void *hip_stream);
+
+/* A buffer of any length (allocate_metal_buffer's size is an int), for workspaces and for tensors above 2 GiB.  Freed
+ * with deallocate_metal_buffer.  0 on failure. */
+uintptr_t gm_allocate_workspace(uintptr_t device, uintptr_t bytes);
+
+/* Dropout's generator state is a 16-byte device buffer of four 32-bit words, {seed, seed, step, 0}, written by the
+ * caller (copy_int32_array_to_metal_buffer) and advanced on the device, once a training step: the kernels read it when
+ * they run, so a captured step draws new masks at every replay.  The mask of an element is a function of (seeds, step,
+ * site, the element's index) alone: Philox4x32-10 with the counter (i / 8 as two words, site, step) gives eight elements
+ * sixteen bits each; an element is kept when its bits reach round(65536 p).  `site` tells the places of a model apart.
+ * The forward and the backward pass of one step use the same state and site. */
+int gm_rng_state_advance(uintptr_t device, uintptr_t command_queue, uintptr_t rng_state);
+
+/* output = keep ? input / (1 - p) : 0, plus the residual (0: none).  The backward pass is the same call on the gradient,
+ * without a residual.  1 / (1 - p) is 65536 / (65536 - round(65536 p)): the mean is kept exactly.  output may be input or
+ * residual.  A dropped element is 0 whatever it was (NaN too); p = 1 drops all, p = 0 needs no state. */
+int execute_dropout(uintptr_t device, uintptr_t command_queue, uintptr_t input_buffer, uintptr_t residual_buffer,
+                    uintptr_t output_buffer, int num_elements, int data_type, float probability, uintptr_t rng_state, int site);
+
+/* output[i, :] = scale * table[tokens[i], :], then dropout (element i * dim + c of `dropout_site`) if the probability is
+ * above 0.  tokens: 32-bit; one outside [0, vocab_size) is padding and gives a row of zeros. */
+int execute_embedding_lookup(uintptr_t device, uintptr_t command_queue, uintptr_t table_buffer, uintptr_t token_buffer,
+                             uintptr_t output_buffer, int num_tokens, int vocab_size, int dim, int table_stride,
+                             int output_stride, int data_type, float scale, float dropout_probability, uintptr_t rng_state,
+                             int dropout_site);
+
+/* The lookup's gradient: row v of the table's gradient is scale times the sum, in the order of the positions, of the
+ * output gradients (through the same dropout) at every position that names v; fp32 sums, rounded once.  Tokens outside
+ * the vocabulary and padding_token (-1: none) give nothing.  accumulate 0: every row is written, those that no token
+ * names with zeros; otherwise the sums are added to what the buffer holds and other rows are not touched (gradient
+ * accumulation, or a table tied to the output layer).  gradient_type: Float32, or data_type.
+ * workspace: gm_embedding_gradient_workspace bytes, aligned to 256. */
+uintptr_t gm_embedding_gradient_workspace(int num_tokens, int vocab_size, int dim);
+int execute_embedding_gradient(uintptr_t device, uintptr_t command_queue, uintptr_t output_gradient_buffer,
+                               uintptr_t token_buffer, uintptr_t table_gradient_buffer, int num_tokens, int vocab_size, int dim,
+                               int output_gradient_stride, int table_gradient_stride, int data_type, int gradient_type,
+                               float scale, int padding_token, int accumulate, float dropout_probability, uintptr_t rng_state,
+                               int dropout_site, uintptr_t workspace, uintptr_t workspace_bytes);
+
+/* Softmax cross entropy of a linear output layer, logits = hidden weight^T (hidden [num_tokens, dim], weight
+ * [vocab_size, dim]), and its gradients, without the logits in memory.
+ *   losses[i] = log(sum over v of exp(logits[i, v])) - logits[i, target[i]], fp32; 0 for a token that does not count:
+ *               its target is ignore_index or no word of the vocabulary.  What stands in such a token's hidden row
+ *               (NaN, too) reaches nothing, and its row of the hidden gradient is 0.
+ *   loss[0]   = their sum, or (mean) the sum over the number that count; 0 when none does.  loss[1] = that number.
+ *   hidden_gradient [num_tokens, dim] in data_type, weight_gradient [vocab_size, dim] in gradient_type (Float32, or
+ *               data_type): gradients of loss[0] times gradient_scale times the loss scale of amp_state (0: none), which is
+ *               read on the device when the call runs.  Either handle may be 0; both: the loss alone.  A gradient that
+ *               overflows its type is +-inf, which the mixed-precision step drops.
+ *   accumulate: the weight gradient is added to what its buffer holds.
+ * With a Float32 gradient_type the slope of the softmax is carried in two 16-bit parts (2^-17 of it and better); with a
+ * 16-bit one it is rounded to that type once.  Float32 tensors are multiplied as three bfloat16 parts each, with
+ * products down to 2^-16 of the largest: about fp32's own accuracy for values below 3.3e38.
+ * workspace: gm_linear_cross_entropy_workspace bytes are enough for the fastest form; anything from
+ * gm_linear_cross_entropy_least_workspace on works, with fewer tokens at a time.  Aligned to 1024.  Both take the weight's
+ * handle and stride because rows that the kernels can take as they lie (16-bit, dim a multiple of 64, stride of 8, base
+ * of 16 bytes) need no copy; handle 0 is the size that always does.  0: sizes that are not offered (more than 2^24 tokens
+ * or words, dim above 2^20).
+ * None of the outputs may overlap an input. */
+uintptr_t gm_linear_cross_entropy_workspace(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer, int weight_stride,
+                                            int data_type, int gradient_type, int with_gradients);
+uintptr_t gm_linear_cross_entropy_least_workspace(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer,
+                                                  int weight_stride, int data_type, int gradient_type, int with_gradients);
+int execute_linear_cross_entropy(uintptr_t device, uintptr_t command_queue, uintptr_t hidden_buffer, uintptr_t weight_buffer,
+                                 uintptr_t target_buffer, uintptr_t losses_buffer, uintptr_t loss_buffer,
+                                 uintptr_t hidden_gradient_buffer, uintptr_t weight_gradient_buffer, int num_tokens,
+                                 int vocab_size, int dim, int hidden_stride, int weight_stride, int hidden_gradient_stride,
+                                 int weight_gradient_stride, int data_type, int gradient_type, int ignore_index, int mean,
+                                 float gradient_scale, uintptr_t amp_state, int accumulate, uintptr_t workspace,
+                                 uintptr_t workspace_bytes);
+
 /* Measurement helpers used by the benchmark and the profiles. */
 
 /* Records a start / stop event pair on the device's stream; gm_timer_stop
