@@ -474,7 +474,8 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.width = (int)up((size_t)dim, kStepK), s.padded = (int)up((size_t)vocab, kStepK);
     s.operand_type = data_type == kFloat32 ? kBFloat16 : data_type;
     s.planes = data_type == kFloat32 ? 3 : 1;
-    s.slope_planes = data_type == kFloat32 ? 3 : gradient_type == kFloat32 ? 2 : 1;
+    // an fp32 gradient of 16-bit activations: as many parts of dS as leave nothing that fp32 sums would notice
+    s.slope_planes = gradient_type != kFloat32 ? 1 : data_type == kFloat16 ? 2 : 3;
     s.keep = !gradients ? kKeepNothing : s.slope_planes == 1 ? kKeepHalf : kKeepFloat;
     s.pack_weights = data_type == kFloat32 || !weights_fit;
     const size_t entry = s.keep == kKeepNothing ? 0 : s.keep == kKeepHalf ? 2 : 4 + 2 * s.slope_planes;
@@ -501,7 +502,7 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     size_t at = 0;
     const auto take = [&](size_t bytes) {
         const size_t here = at;
-        at += up(bytes, 1024);
+        at += up(bytes, 256);
         return here;
     };
     s.head = take(sizeof(LossHead));
@@ -531,15 +532,15 @@ static bool fitting_plan(LossPlan &s, size_t bytes, int n, int vocab, int dim, b
 
 static bool weights_fit(uintptr_t weight, int dim, int stride, int data_type)
 {
-    return data_type != kFloat32 && weight != 0 && weight % 16 == 0 && dim % kStepK == 0 && stride % 8 == 0;
+    return data_type != kFloat32 && weight != 0 && weight % 16 == 0 && dim % kStepK == 0 && stride % 8 == 0 && stride <= 1 << 22;
 }
 
 static constexpr PlanePairs kOnePair = {1, 0x0};
 // fp32 by three planes of eight bits: the six products of 2^-16 and more, the small ones first
 // (codes: P plane + 4 Q plane)
 static constexpr PlanePairs kSixPairs = {6, 0x041528};
-// x (one plane) with dS (two): the rest first
-static constexpr PlanePairs kSlopePairs = {2, 0x04};
+// x (one plane) with the parts of dS: the smallest first
+static constexpr PlanePairs kTwoSlopes = {2, 0x04}, kThreeSlopes = {3, 0x048};
 
 struct LossCall {
     uintptr_t hidden, weight, targets, losses, loss, dx, dw;
@@ -624,7 +625,7 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
         if (c.dw) {
             ProductArgs a{};
             a.p = xs, a.p.rows = s.dim, a.q = slopes, a.q.rows = s.vocab;
-            a.pairs = s.planes == 3 ? kSixPairs : s.slope_planes == 2 ? kSlopePairs : kOnePair;
+            a.pairs = s.planes == 3 ? kSixPairs : s.slope_planes == 3 ? kThreeSlopes : s.slope_planes == 2 ? kTwoSlopes : kOnePair;
             a.first = first, a.most = tokens, a.splits = 1, a.head = head, a.unscale = 1.0f / kSlopeScale<T>;
             const bool last = k + 1 == s.chunks;
             float *sums = reinterpret_cast<float *>(space + s.sums);
@@ -646,7 +647,7 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
 
 static bool loss_sizes(int n, int vocab, int dim, int data_type, int gradient_type)
 {
-    return n >= 0 && n <= 1 << 24 && vocab > 0 && vocab <= 1 << 24 && dim > 0 && dim <= 1 << 20 && known_type(data_type) &&
+    return n >= 0 && n <= 1 << 24 && vocab > 0 && vocab <= 1 << 22 && dim > 0 && dim <= 1 << 20 && known_type(data_type) &&
            (gradient_type == kFloat32 || gradient_type == data_type);
 }
 
@@ -706,8 +707,8 @@ try {
     LossPlan plan;
     if (!fitting_plan(plan, workspace ? (size_t)workspace_bytes : 0, num_tokens, vocab_size, dim,
                       weights_fit(weight_buffer, dim, weight_stride, data_type), data_type, gradient_type, gradients) ||
-        workspace % 1024 != 0 || !rows_fit("workspace", workspace, 1, plan.bytes, plan.bytes, 1)) {
-        set_error("the workspace holds %zu bytes (or is not aligned to 1024): at least %zu are needed", (size_t)workspace_bytes, plan.bytes);
+        workspace % 256 != 0 || !rows_fit("workspace", workspace, 1, plan.bytes, plan.bytes, 1)) {
+        set_error("the workspace holds %zu bytes (or is not aligned to 256): at least %zu are needed", (size_t)workspace_bytes, plan.bytes);
         return kRcWorkspace;
     }
     Context *ctx = resolve_device(device);

@@ -13,6 +13,8 @@
 
 #include "gm_ops.hpp"
 
+#include <type_traits>
+
 namespace gm {
 
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -63,45 +65,81 @@ struct Tile {
 
     __device__ static inline int across_swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) & (kPieces - 1); }
 
-    // This lane's source addresses for one step, k0 the step's first k, `limit` the k that exist (across).
-    __device__ static inline void load(const Operand &op, const short *plane, int row0, int k0, int limit, uint32_t lds, int wave, int lane)
+    // Byte offsets of this lane's loads from the tile's first k of row 0, rows behind the last one replaced by it.
+    __device__ static inline void offsets(const Operand &op, int row0, int wave, int lane, uint32_t (&out)[kLoads])
     {
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
             const int at = (i * WAVES + wave) * 1024 + lane * 16;      // byte of the tile this lane fills
-            const short *src;
             if (!ACROSS) {
                 const int row = at / 128, piece = ((at / 16) & 7) ^ (row & 7);
-                const int r = row0 + row < op.rows ? row0 + row : op.rows - 1;
-                src = plane + (int64_t)r * op.stride + k0 + piece * 8;
+                const int r = row0 + row < op.rows ? row : op.rows - 1 - row0;
+                out[i] = (uint32_t)r * (uint32_t)op.stride * 2u + piece * 16;
             } else {
                 const int k = at / (ROWS * 2), half = (at / 16) & 1, group = ((at / 32) & (kPieces - 1)) ^ across_swizzle(k);
-                const int last = (op.rows - 1) & ~7;      // (rows are there in eights)
-                int r = row0 + group * 16 + half * 8;
-                r = r < last ? r : last;
-                const int kk = k0 + k < limit ? k0 + k : limit - 1;
-                src = plane + (int64_t)kk * op.stride + r;
+                const int last = (op.rows - 1) & ~7;                   // (rows are there in eights)
+                const int r = row0 + group * 16 + half * 8;
+                out[i] = (uint32_t)k * (uint32_t)op.stride * 2u + (uint32_t)((r < last ? r : last) - row0) * 2u;
             }
-            const uint32_t to = lds + (i * WAVES + wave) * 1024;
-            // (m0 takes the wavefront's LDS address; one wait state lies between its write and its use)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src) : "memory");
         }
     }
 
-    // The fragment of rows row .. row + 15, k half * 32 .. + 31: lane l has row l % 16, k 8 (l / 16) .. + 7 of them.
-    __device__ static inline s16x8 fragment(uint32_t lds, int row, int half, int lane)
+    // The last step of a sum that is no whole number of steps: `there` of its k exist, the others become the last one again
+    // (across; along, rows are whole steps long).
+    __device__ static inline void clamp(int there, uint32_t stride_bytes, int wave, int lane, uint32_t (&out)[kLoads])
     {
-        if (!ACROSS) {
-            const int r = row + (lane & 15), c = half * 4 + (lane >> 4);
-            return *reinterpret_cast<const GM_LDS s16x8 *>(lds + r * 128 + ((c ^ (r & 7)) << 4));
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const int k = ((i * WAVES + wave) * 1024 + lane * 16) / (ROWS * 2);
+            if (k >= there) out[i] -= (uint32_t)(k - there + 1) * stride_bytes;
         }
+    }
+
+    // The wavefront's i-th load of a step.  `base`: the tile's first k of row 0.
+    __device__ static inline void load(const char *base, uint32_t offset, uint32_t lds, int wave, int i)
+    {
+        // (m0 takes the wavefront's LDS address; one wait state lies between its write and its use)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + (i * WAVES + wave) * 1024), "v"(offset),
+                     "s"(base)
+                     : "memory");
+    }
+
+    // Where this lane reads the fragments of the wavefront's rows row .. row + 16 N - 1: lane l has row l % 16 and k 8 (l / 16)
+    // .. + 7 of a half.  Along, the fragments of a half lie a constant apart; across, every sixteen rows have a place.
+    template <int N>
+    struct Places {
+        uint32_t at[ACROSS ? N : 2];
+    };
+    template <int N>
+    __device__ static inline Places<N> places(uint32_t lds, int row, int lane)
+    {
+        Places<N> out;
+        if (!ACROSS) {
+            const int r = row + (lane & 15);
+#pragma unroll
+            for (int half = 0; half < 2; half++) out.at[half] = lds + r * 128 + (((half * 4 + (lane >> 4)) ^ (r & 7)) << 4);
+        } else {
+            const int k = (lane >> 4) * 8 + ((lane & 15) >> 2);
+#pragma unroll
+            for (int i = 0; i < N; i++) out.at[ACROSS ? i : 0] = lds + k * (ROWS * 2) + (((row / 16 + i) ^ across_swizzle(k)) << 5) + (lane & 3) * 8;
+        }
+        return out;
+    }
+    template <int N>
+    __device__ static inline void move(Places<N> &places, uint32_t bytes)      // to the next stage
+    {
+#pragma unroll
+        for (int i = 0; i < (ACROSS ? N : 2); i++) places.at[i] += bytes;
+    }
+    template <int N>
+    __device__ static inline s16x8 fragment(const Places<N> &places, int i, int half)
+    {
+        if (!ACROSS) return *reinterpret_cast<const GM_LDS s16x8 *>(places.at[half] + (uint32_t)(i * 2048));
         s16x8 out;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int k = half * 32 + (lane >> 4) * 8 + j * 4 + ((lane & 15) >> 2);
-            const int group = (row >> 4) ^ across_swizzle(k);
             const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                reinterpret_cast<GM_LDS s16x4 *>(lds + k * (ROWS * 2) + (group << 5) + (lane & 3) * 8));
+                reinterpret_cast<GM_LDS s16x4 *>(places.at[ACROSS ? i : 0] + (uint32_t)(half * (32 * ROWS * 2) + j * (4 * ROWS * 2))));
 #pragma unroll
             for (int e = 0; e < 4; e++) out[j * 4 + e] = v[e];
         }
@@ -133,48 +171,133 @@ struct Shape {
 
 // The sum over steps [first, last) of the pairs' k; acc[i][j]: rows 16 i of P, 16 j of Q of this wavefront.
 // steps: steps of one pair; limit_p / limit_q: the k that exist where an operand lies across.
+//
+// A step's matrix instructions come in two halves of 32 k, row by row of P's fragments.  A fragment of P is replaced by
+// the next half's as soon as its row is through, so reads from LDS run half a step ahead all the time.  Shortly after the
+// first half every wavefront has read all of its stage: one barrier there frees the stage for the loads of the step
+// STAGES later, and makes the next step's data, which have arrived by then, visible.
 template <typename T, typename S, bool PACROSS, bool QACROSS>
 __device__ inline void multiply_tiles(const Operand &p, const Operand &q, const PlanePairs &pairs, int p0, int q0, int steps, int limit_p,
                                       int limit_q, int first, int last, uint32_t lds, f32x4 (&acc)[S::MP][S::MQ])
 {
     typedef Tile<S::BP, PACROSS, S::WAVES> TP;
     typedef Tile<S::BQ, QACROSS, S::WAVES> TQ;
+    constexpr int kLoads = TP::kLoads + TQ::kLoads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
+    const uint32_t lds_q = lds + S::STAGES * TP::kBytes;      // P's stages, then Q's
+    uint32_t off_p[TP::kLoads], off_q[TQ::kLoads];
+    TP::offsets(p, p0, wave, lane, off_p);
+    TQ::offsets(q, q0, wave, lane, off_q);
+    auto at_p = TP::template places<S::MP>(lds, wp, lane);
+    auto at_q = TQ::template places<S::MQ>(lds_q, wq, lane);
 #pragma unroll
     for (int i = 0; i < S::MP; i++)
 #pragma unroll
         for (int j = 0; j < S::MQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const auto load = [&](int step) {      // beyond the last step the last one again, into a stage that nobody reads
-        const int s = step < last ? step : last - 1;
-        const int pair = s / steps, k0 = (s - pair * steps) * kStepK;
-        const uint32_t code = pairs.codes >> (4 * pair);
-        const uint32_t at = lds + (uint32_t)((step - first) % S::STAGES) * (TP::kBytes + TQ::kBytes);
-        TP::load(p, p.base + (int64_t)(code & 3) * p.plane, p0, k0, limit_p, at, wave, lane);
-        TQ::load(q, q.base + (int64_t)(code >> 2 & 3) * q.plane, q0, k0, limit_q, at + TP::kBytes, wave, lane);
+    // the next step to load: its pair, its k, its addresses
+    int load_step = first, load_pair = first / steps, load_k = (first - load_pair * steps) * kStepK;
+    const int edge = (steps - 1) * kStepK;      // the k of a pair's last step
+    const int64_t ahead_p = PACROSS ? (int64_t)p.stride * (2 * kStepK) : 2 * kStepK, ahead_q = QACROSS ? (int64_t)q.stride * (2 * kStepK) : 2 * kStepK;
+    const char *from_p, *from_q;
+    const auto seek = [&]() {
+        const uint32_t code = pairs.codes >> (4 * load_pair);
+        const short *bp = p.base + (int64_t)(code & 3) * p.plane, *bq = q.base + (int64_t)(code >> 2 & 3) * q.plane;
+        from_p = reinterpret_cast<const char *>(PACROSS ? bp + (int64_t)load_k * p.stride + p0 : bp + (int64_t)p0 * p.stride + load_k);
+        from_q = reinterpret_cast<const char *>(QACROSS ? bq + (int64_t)load_k * q.stride + q0 : bq + (int64_t)q0 * q.stride + load_k);
     };
-    for (int s = 0; s < S::STAGES - 1; s++) load(first + s);
-    for (int step = first; step < last; step++) {
-        // this step's loads have arrived (those of the later stages may be on their way), and every wavefront is done
-        // with the stage that is filled next
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::STAGES - 2) * (TP::kLoads + TQ::kLoads)) : "memory");
-        __builtin_amdgcn_s_barrier();
-        load(step + S::STAGES - 1);
-        const uint32_t at = lds + (uint32_t)((step - first) % S::STAGES) * (TP::kBytes + TQ::kBytes);
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            s16x8 fp[S::MP], fq[S::MQ];
-#pragma unroll
-            for (int j = 0; j < S::MQ; j++) fq[j] = TQ::fragment(at + TP::kBytes, wq + j * 16, half, lane);
-#pragma unroll
-            for (int i = 0; i < S::MP; i++) fp[i] = TP::fragment(at, wp + i * 16, half, lane);
-#pragma unroll
-            for (int i = 0; i < S::MP; i++)
-#pragma unroll
-                for (int j = 0; j < S::MQ; j++) acc[i][j] = multiply_add<T>(fp[i], fq[j], acc[i][j]);
+    const auto at_edge = [&]() {
+        if (PACROSS && limit_p < edge + kStepK) TP::clamp(limit_p - edge, (uint32_t)p.stride * 2u, wave, lane, off_p);
+        if (QACROSS && limit_q < edge + kStepK) TQ::clamp(limit_q - edge, (uint32_t)q.stride * 2u, wave, lane, off_q);
+    };
+    seek();
+    if (load_k == edge) at_edge();
+    const auto load_one = [&](int stage, int i) {      // i: which of this wavefront's loads
+        if (i < TP::kLoads) TP::load(from_p, off_p[i < TP::kLoads ? i : 0], lds + stage * TP::kBytes, wave, i);
+        else TQ::load(from_q, off_q[i >= TP::kLoads ? i - TP::kLoads : 0], lds_q + stage * TQ::kBytes, wave, i - TP::kLoads);
+    };
+    const auto loaded = [&]() {
+        load_step++;
+        load_k += kStepK;
+        from_p += ahead_p;
+        from_q += ahead_q;
+        if (load_k >= edge) {
+            if (load_k > edge) {      // the next pair from its beginning
+                load_k = 0;
+                if (++load_pair < pairs.count) {
+                    seek();
+                    if (PACROSS && limit_p < edge + kStepK) TP::offsets(p, p0, wave, lane, off_p);
+                    if (QACROSS && limit_q < edge + kStepK) TQ::offsets(q, q0, wave, lane, off_q);
+                }
+            }
+            if (load_k == edge) at_edge();
         }
-    }
+    };
+#pragma unroll
+    for (int s = 0; s < S::STAGES; s++)
+        if (load_step < last) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) load_one(s, i);
+            loaded();
+        }
+    if (first + S::STAGES <= last) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S::STAGES - 1) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+
+    s16x8 fp[S::MP], fq[2][S::MQ];
+    constexpr int kMeet = S::MP >= 4 ? 1 : 0;      // the row of the second half that the barrier follows
+    // The order is pinned (sched_barrier): left to itself the compiler gathers the reads in front of their first use, and the
+    // matrix cores wait for them.
+    const auto row = [&](int half, int i) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < S::MQ; j++) acc[i][j] = multiply_add<T>(fp[i], fq[half][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int stage = 0;
+    // `more`: a step is left to load, and all stages are under way
+    const auto whole_step = [&](auto more) {
+#pragma unroll
+        for (int i = 0; i < S::MP; i++) {      // the first half; the second one's fragments are read
+            row(0, i);
+#pragma unroll
+            for (int j = i * S::MQ / S::MP; j < (i + 1) * S::MQ / S::MP; j++) fq[1][j] = TQ::fragment(at_q, j, 1);
+            fp[i] = TP::fragment(at_p, i, 1);
+        }
+        const bool wraps = stage == S::STAGES - 1;
+        TP::move(at_p, wraps ? -(S::STAGES - 1) * TP::kBytes : TP::kBytes);
+        TQ::move(at_q, wraps ? -(S::STAGES - 1) * TQ::kBytes : TQ::kBytes);
+#pragma unroll
+        for (int i = 0; i < S::MP; i++) {      // the second half; the next step's first half is read
+            row(1, i);
+            if (i < kMeet) continue;
+            if (i == kMeet) {
+                if constexpr (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::STAGES - 2) * kLoads) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+            }
+            constexpr int kRows = S::MP - kMeet;
+            const int at = i - kMeet;
+#pragma unroll
+            for (int j = at * S::MQ / kRows; j < (at + 1) * S::MQ / kRows; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
+#pragma unroll
+            for (int r = i == kMeet ? 0 : i; r <= i; r++) fp[r] = TP::fragment(at_p, r, 0);
+            if constexpr (more) {
+#pragma unroll
+                for (int l = at * kLoads / kRows; l < (at + 1) * kLoads / kRows; l++) load_one(stage, l);
+            }
+        }
+        if constexpr (more) loaded();
+        stage = wraps ? 0 : stage + 1;
+    };
+#pragma unroll
+    for (int j = 0; j < S::MQ; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
+#pragma unroll
+    for (int i = 0; i < S::MP; i++) fp[i] = TP::fragment(at_p, i, 0);
+    int step = first;
+    for (; step + S::STAGES < last; step++) whole_step(std::true_type());
+    for (; step < last; step++) whole_step(std::false_type());
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 

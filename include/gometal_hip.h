@@ -469,14 +469,14 @@ int execute_embedding_gradient(uintptr_t device, uintptr_t command_queue, uintpt
  *               read on the device when the call runs.  Either handle may be 0; both: the loss alone.  A gradient that
  *               overflows its type is +-inf, which the mixed-precision step drops.
  *   accumulate: the weight gradient is added to what its buffer holds.
- * With a Float32 gradient_type the slope of the softmax is carried in two 16-bit parts (2^-17 of it and better); with a
- * 16-bit one it is rounded to that type once.  Float32 tensors are multiplied as three bfloat16 parts each, with
+ * With a Float32 gradient_type the slope of the softmax is carried in 16-bit parts (two of Float16, three of BFloat16:
+ * 22 bits and more); with a 16-bit one it is rounded to that type once.  Float32 tensors are multiplied as three bfloat16 parts each, with
  * products down to 2^-16 of the largest: about fp32's own accuracy for values below 3.3e38.
  * workspace: gm_linear_cross_entropy_workspace bytes are enough for the fastest form; anything from
- * gm_linear_cross_entropy_least_workspace on works, with fewer tokens at a time.  Aligned to 1024.  Both take the weight's
+ * gm_linear_cross_entropy_least_workspace on works, with fewer tokens at a time.  Aligned to 256.  Both take the weight's
  * handle and stride because rows that the kernels can take as they lie (16-bit, dim a multiple of 64, stride of 8, base
- * of 16 bytes) need no copy; handle 0 is the size that always does.  0: sizes that are not offered (more than 2^24 tokens
- * or words, dim above 2^20).
+ * of 16 bytes) need no copy; handle 0 is the size that always does.  0: sizes that are not offered (more than 2^24 tokens, 2^22
+ * words, or a dim above 2^20).
  * None of the outputs may overlap an input. */
 uintptr_t gm_linear_cross_entropy_workspace(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer, int weight_stride,
                                             int data_type, int gradient_type, int with_gradients);

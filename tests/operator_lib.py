@@ -116,7 +116,7 @@ class Buffers:
     def state(self, words=(1234567, 0x89ABCDEF, 3, 0)):
         return self.put(np.array(words, np.uint32))
 
-    def space(self, nbytes, align=1024):
+    def space(self, nbytes, align=256):
         """A workspace of exactly that many bytes, filled with NaN patterns."""
         raw = np.full(nbytes + 2 * self.BORDER, 0xFF, np.uint8)
         h = self.dev.from_numpy(raw)

@@ -31,7 +31,7 @@ def gradient(lib, device=DEVICE, dy=A, tokens=B, g=C, n=4, v=10, d=8, ys=8, gs=8
 
 
 def loss(lib, device=DEVICE, x=A, w=B, target=C, losses=D, total=D, dx=0x50000, dw=0x60000, n=4, v=10, d=8, xs=8, ws=8, dxs=8, dws=8,
-         t=2, o=2, amp=0, space=0x70000 * 1024, size=1 << 30):
+         t=2, o=2, amp=0, space=0x70000, size=1 << 30):
     return lib.execute_linear_cross_entropy(device, 0, x, w, target, losses, total, dx, dw, n, v, d, xs, ws, dxs, dws, t, o, -100, 1,
                                             1.0, amp, 0, space, size)
 
@@ -78,10 +78,10 @@ def test_table_gradient_workspace(lib):
 
 @pytest.mark.parametrize("change, code", [
     (dict(device=0), -1), (dict(x=0), -4), (dict(w=0), -4), (dict(target=0), -4), (dict(losses=0), -4), (dict(total=0), -4),
-    (dict(n=-1), -5), (dict(n=2 ** 24 + 1), -5), (dict(v=0), -5), (dict(v=2 ** 24 + 1), -5), (dict(d=0), -5), (dict(xs=7), -5),
+    (dict(n=-1), -5), (dict(n=2 ** 24 + 1), -5), (dict(v=0), -5), (dict(v=2 ** 22 + 1), -5), (dict(d=0), -5), (dict(xs=7), -5),
     (dict(ws=7), -5), (dict(dxs=7), -5), (dict(dws=7), -5), (dict(t=1), -19), (dict(t=2, o=4), -19), (dict(t=0, o=2), -19),
     (dict(x=A + 1), -5), (dict(w=B + 1), -5), (dict(target=C + 2), -5), (dict(dx=0x50001), -5), (dict(dw=0x60001), -5),
-    (dict(space=0), -18), (dict(space=0x70100), -18), (dict(size=1000), -18)])
+    (dict(space=0), -18), (dict(space=0x70080), -18), (dict(size=1000), -18)])
 def test_loss(lib, change, code):
     assert loss(lib, **change) == code
 
