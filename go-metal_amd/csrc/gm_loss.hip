@@ -35,7 +35,7 @@ constexpr int kShapeP[3] = {256, 128, 128}, kShapeQ[3] = {256, 128, 32}, kShapeS
 
 // exp(s - m) in 16 bits is 32768 times itself in fp16, dS of fp16 operands 16384 times itself: both keep clear of the
 // subnormals (down to 2^-29 and 2^-28), and an entry's rounding is 2^-12 of it.
-constexpr float kExpScale = 32768.0f;
+constexpr float kExpScale = 32768.0f, kExpShift = 15.0f;
 template <typename T>
 constexpr float kSlopeScale = 1.0f;
 template <>
@@ -117,17 +117,17 @@ constexpr int kPackBlock = 256;
 template <typename I, typename T>
 __global__ void __launch_bounds__(kPackBlock)
 pack_tokens_kernel(const I *x, int64_t x_stride, int n, int dim, int width, const LossHead *head, const int *place_of, T *packed,
-                   int64_t plane, int planes, float *losses, I *dx, int64_t dx_stride)
+                   int64_t packed_stride, int64_t plane, int planes, float *losses, I *dx, int64_t dx_stride)
 {
     const int i = blockIdx.x;
     if (i >= n) {
         const int r = head->count + (i - n), end = (head->count + kStepK - 1) / kStepK * kStepK;
-        if (r < end) pack_row<I, T>(nullptr, packed + (int64_t)r * width, 0, width, plane, planes);
+        if (r < end) pack_row<I, T>(nullptr, packed + r * packed_stride, 0, width, plane, planes);
         return;
     }
     const int place = place_of[i];
     if (place >= 0) {
-        pack_row<I, T>(x + (int64_t)i * x_stride, packed + (int64_t)place * width, dim, width, plane, planes);
+        pack_row<I, T>(x + (int64_t)i * x_stride, packed + place * packed_stride, dim, width, plane, planes);
         return;
     }
     if (threadIdx.x == 0) losses[i] = 0.0f;
@@ -154,7 +154,8 @@ struct LogitsArgs {
     float *target_logit;
     float2 *stats;              // [row of the chunk][group]: maximum, sum of exp(s - maximum)
     int groups, keep;
-    void *kept;                 // [row of the chunk][padded]
+    void *kept;                 // [row of the chunk][stride]
+    int64_t stride;
 };
 
 template <typename T, typename S>
@@ -173,45 +174,59 @@ logits_kernel(LogitsArgs a)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wp = p0 + wave / S::WQ * (S::BP / S::WP) + (lane >> 4) * 4, wq = q0 + wave % S::WQ * (S::BQ / S::WQ) + (lane & 15);
     const int group = (p0 + wave / S::WQ * (S::BP / S::WP)) / (S::BP / S::WP);
+    const bool ragged = p0 + S::BP > a.vocab;
 #pragma unroll
     for (int j = 0; j < S::MQ; j++) {
         const int q = wq + j * 16;
         const bool there = q < rows;
-        const int target = there ? a.row_target[a.first + q] : -1;
+        // the target's logit, if it is one of this lane's: words wp + 16 i + (0 .. 3)
+        const int at = (there ? a.row_target[a.first + q] : -1) - wp;
+        if (at >= 0 && at < S::MP * 16 && (at & 15) < 4) {
+            float logit = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S::MP; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) logit = at == i * 16 + r ? acc[i][j][r] : logit;
+            a.target_logit[a.first + q] = logit;
+        }
+        if (ragged) {
+#pragma unroll
+            for (int i = 0; i < S::MP; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[i][j][r] = wp + i * 16 + r < a.vocab ? acc[i][j][r] : -INFINITY;
+        }
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < S::MP; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int p = wp + i * 16 + r;
-                if (p >= a.vocab) acc[i][j][r] = -INFINITY;
-                top = fmaxf(top, acc[i][j][r]);
-                if (p == target) a.target_logit[a.first + q] = acc[i][j][r];
-            }
+        for (int i = 0; i < S::MP; i++) top = fmaxf(fmaxf(fmaxf(top, acc[i][j][0]), acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3]));
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float ref = top == -INFINITY ? 0.0f : top;      // (a share that lies behind the vocabulary: all zeros)
         float sum = 0.0f;
+        const int64_t row = q * a.stride;
+        if (a.keep == kKeepFloat) {
 #pragma unroll
-        for (int i = 0; i < S::MP; i++) {
-            f32x4 e;
+            for (int i = 0; i < S::MP; i++) {
+                f32x4 e;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                e[r] = a.keep == kKeepFloat ? expf(acc[i][j][r] - ref) : __expf(acc[i][j][r] - ref);
-                sum += e[r];
+                for (int r = 0; r < 4; r++) sum += e[r] = expf(acc[i][j][r] - ref);
+                if (there && wp + i * 16 < a.padded) *reinterpret_cast<f32x4 *>(static_cast<float *>(a.kept) + row + wp + i * 16) = e;
             }
-            const int p = wp + i * 16;
-            if (a.keep == kKeepNothing || !there || p >= a.padded) continue;
-            const int64_t at = (int64_t)q * a.padded + p;
-            if (a.keep == kKeepFloat) {
-                *reinterpret_cast<f32x4 *>(static_cast<float *>(a.kept) + at) = e;
-            } else {
-                typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+        } else {
+            // 2^15 exp(s - ref) by the hardware's power of two; the sum's factor is taken out again exactly
+            typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int i = 0; i < S::MP; i++) {
                 f16x4 h;
 #pragma unroll
-                for (int r = 0; r < 4; r++) h[r] = (_Float16)(e[r] * kExpScale);
-                *reinterpret_cast<f16x4 *>(static_cast<_Float16 *>(a.kept) + at) = h;
+                for (int r = 0; r < 4; r++) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r] - ref, 1.44269504f, kExpShift));
+                    sum += e;
+                    h[r] = (_Float16)e;
+                }
+                if (a.keep == kKeepHalf && there && wp + i * 16 < a.padded)
+                    *reinterpret_cast<f16x4 *>(static_cast<_Float16 *>(a.kept) + row + wp + i * 16) = h;
             }
+            sum *= 1.0f / kExpScale;
         }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
@@ -231,7 +246,7 @@ struct RowsArgs {
     float *losses;
     int keep, planes;
     void *kept, *slopes;       // kKeepHalf: the same memory
-    int64_t plane;
+    int64_t stride, plane;
 };
 
 __device__ inline float block_reduce(float x, bool maximum, float *scratch)
@@ -256,7 +271,7 @@ rows_kernel(RowsArgs a)
 {
     __shared__ float scratch[kRowBlock / 64];
     const int rows = chunk_rows(a.head, a.first, a.most), r = blockIdx.x;
-    T *slopes = static_cast<T *>(a.slopes) + (int64_t)r * a.padded;
+    T *slopes = static_cast<T *>(a.slopes) + r * a.stride;
     const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (r >= rows) {
         if (a.keep != kKeepNothing && r < (rows + kStepK - 1) / kStepK * kStepK)      // a whole step of k for dW
@@ -280,10 +295,10 @@ rows_kernel(RowsArgs a)
         float v[8];
         float f = c < a.vocab ? expf(stats[c / a.span].x - lse) : 0.0f;
         if (a.keep == kKeepHalf) {
-            load8(static_cast<const _Float16 *>(a.kept) + (int64_t)r * a.padded + c, true, 8, v);
+            load8(static_cast<const _Float16 *>(a.kept) + r * a.stride + c, true, 8, v);
             f = f * (1.0f / kExpScale);
         } else {
-            load8(static_cast<const float *>(a.kept) + (int64_t)r * a.padded + c, true, 8, v);
+            load8(static_cast<const float *>(a.kept) + r * a.stride + c, true, 8, v);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = c + e < a.vocab ? (c + e == target ? at_target : v[e] * f) * kSlopeScale<T> : 0.0f;
@@ -444,12 +459,17 @@ join_splits_kernel(ProductArgs a)
 // Everything that follows from the sizes: what lies where in the workspace, and which shape each product takes.
 struct LossPlan {
     int n, vocab, dim, width, padded, chunk, chunks;
+    int x_stride, slope_stride;            // of the packed tokens and of dS
     int operand_type;                      // kFloat16 or kBFloat16
     int planes, slope_planes, keep;        // planes of x (and W); of dS
     bool gradients, pack_weights, sum_weights;      // sum_weights: dW of several chunks in 16 bits needs fp32 sums
     int logits_shape, groups, dx_shape, dx_splits, dw_shape;
     size_t head, row_of, place_of, row_target, target_logit, x, w, stats, kept, slopes, partial, sums, bytes;
 };
+
+// Rows that the kernels lay out themselves are 128 bytes longer than their contents: a step reads 128 bytes of 256 rows, and
+// rows a large power of two apart would all lie on the same channel of the L2.
+constexpr int kSkew = 64;
 
 constexpr int kLeastChunk = 256;
 constexpr size_t kKeptBytes = (size_t)4 << 30;      // of exp(s - m) and dS together, unless one chunk needs more
@@ -472,6 +492,7 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     LossPlan s{};
     s.n = n, s.vocab = vocab, s.dim = dim, s.gradients = gradients;
     s.width = (int)up((size_t)dim, kStepK), s.padded = (int)up((size_t)vocab, kStepK);
+    s.x_stride = s.width + kSkew, s.slope_stride = s.padded + kSkew;
     s.operand_type = data_type == kFloat32 ? kBFloat16 : data_type;
     s.planes = data_type == kFloat32 ? 3 : 1;
     // an fp32 gradient of 16-bit activations: as many parts of dS as leave nothing that fp32 sums would notice
@@ -480,7 +501,7 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.pack_weights = data_type == kFloat32 || !weights_fit;
     const size_t entry = s.keep == kKeepNothing ? 0 : s.keep == kKeepHalf ? 2 : 4 + 2 * s.slope_planes;
     if (chunk <= 0) {
-        size_t most = entry ? kKeptBytes / (entry * s.padded) / kLeastChunk * kLeastChunk : (size_t)n;
+        size_t most = entry ? kKeptBytes / (entry * s.slope_stride) / kLeastChunk * kLeastChunk : (size_t)n;
         if (most < kLeastChunk) most = kLeastChunk;
         chunk = most < (size_t)n ? (int)most : n;
     }
@@ -507,11 +528,11 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     };
     s.head = take(sizeof(LossHead));
     s.row_of = take(4 * rows), s.place_of = take(4 * rows), s.row_target = take(4 * rows), s.target_logit = take(4 * rows);
-    s.x = take(rows * s.width * 2 * s.planes);
+    s.x = take(rows * s.x_stride * 2 * s.planes);
     s.w = take(s.pack_weights ? (size_t)vocab * s.width * 2 * s.planes : 0);
     s.stats = take(sizeof(float2) * (size_t)s.chunk * s.groups);
-    s.kept = take(s.keep == kKeepNothing ? 0 : chunk_rows * s.padded * (s.keep == kKeepHalf ? 2 : 4));
-    s.slopes = s.keep == kKeepFloat ? take(chunk_rows * s.padded * 2 * s.slope_planes) : s.kept;
+    s.kept = take(s.keep == kKeepNothing ? 0 : chunk_rows * s.slope_stride * (s.keep == kKeepHalf ? 2 : 4));
+    s.slopes = s.keep == kKeepFloat ? take(chunk_rows * s.slope_stride * 2 * s.slope_planes) : s.kept;
     s.partial = take(gradients && s.dx_splits > 1 ? (size_t)s.dx_splits * s.chunk * dim * 4 : 0);
     s.sums = take(s.sum_weights ? (size_t)vocab * dim * 4 : 0);
     s.bytes = at;
@@ -580,12 +601,12 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     T *x = reinterpret_cast<T *>(space + s.x);
     float *losses = reinterpret_cast<float *>(c.losses);
     const size_t rows = ((size_t)s.n + kStepK - 1) / kStepK * kStepK, chunk_rows = ((size_t)s.chunk + kStepK - 1) / kStepK * kStepK;
-    const int64_t x_plane = (int64_t)rows * s.width, w_plane = (int64_t)s.vocab * s.width, slope_plane = (int64_t)chunk_rows * s.padded;
+    const int64_t x_plane = (int64_t)rows * s.x_stride, w_plane = (int64_t)s.vocab * s.width, slope_plane = (int64_t)chunk_rows * s.slope_stride;
 
     scan_targets_kernel<<<1, kScanBlock, 0, stream>>>(reinterpret_cast<const int *>(c.targets), s.n, s.vocab, c.ignore, c.mean,
                                                       c.gradient_scale, c.amp, head, row_of, place_of, row_target);
     pack_tokens_kernel<I, T><<<s.n + kStepK, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.hidden), c.hidden_stride, s.n, s.dim,
-                                                                      s.width, head, place_of, x, x_plane, s.planes, losses,
+                                                                      s.width, head, place_of, x, s.x_stride, x_plane, s.planes, losses,
                                                                       reinterpret_cast<I *>(c.dx), c.dx_stride);
     Operand w{reinterpret_cast<const short *>(c.weight), c.weight_stride, 0, s.vocab};
     if (s.pack_weights) {
@@ -597,19 +618,19 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     for (int k = 0; k < s.chunks; k++) {
         const int first = k * s.chunk, most = s.n - first < s.chunk ? s.n - first : s.chunk;
         if (most <= 0 && k > 0) break;
-        const Operand xs{reinterpret_cast<const short *>(x + (int64_t)first * s.width), s.width, x_plane, 0};
+        const Operand xs{reinterpret_cast<const short *>(x + (int64_t)first * s.x_stride), s.x_stride, x_plane, 0};
         const int tokens = most > 0 ? most : 0;
         LogitsArgs l{w, xs, pairs, s.width / kStepK, first, tokens, s.vocab, s.padded, head, row_target, target_logit,
-                     reinterpret_cast<float2 *>(space + s.stats), s.groups, s.keep, space + s.kept};
+                     reinterpret_cast<float2 *>(space + s.stats), s.groups, s.keep, space + s.kept, s.slope_stride};
         RowsArgs r{first, tokens, s.vocab, s.padded, s.groups, kShapeSpan[s.logits_shape], head, row_of, row_target, target_logit,
                    reinterpret_cast<const float2 *>(space + s.stats), losses, s.keep, s.slope_planes, space + s.kept, space + s.slopes,
-                   slope_plane};
+                   s.slope_stride, slope_plane};
         if (tokens > 0) {
             launch_logits<T>(s.logits_shape, l, tokens, stream);
             rows_kernel<T><<<(tokens + kStepK - 1) / kStepK * kStepK, kRowBlock, 0, stream>>>(r);
         }
         if (!s.gradients) continue;
-        const Operand slopes{reinterpret_cast<const short *>(space + s.slopes), s.padded, slope_plane, 0};
+        const Operand slopes{reinterpret_cast<const short *>(space + s.slopes), s.slope_stride, slope_plane, 0};
         if (c.dx && tokens > 0) {
             ProductArgs a{};
             a.p = w, a.p.rows = s.dim, a.q = slopes, a.pairs = pairs;
