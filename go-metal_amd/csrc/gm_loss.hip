@@ -164,8 +164,8 @@ logits_kernel(LogitsArgs a)
 {
     __shared__ __attribute__((aligned(1024))) char tiles[S::LDS];
     const int rows = chunk_rows(a.head, a.first, a.most);
-    uint32_t tp, tq;
-    if (!tile_of(blockIdx.x, (a.vocab + S::BP - 1) / S::BP, (rows + S::BQ - 1) / S::BQ, 8, tp, tq)) return;
+    uint32_t tp, tq, part;
+    if (!tile_of(blockIdx.x, (a.vocab + S::BP - 1) / S::BP, (rows + S::BQ - 1) / S::BQ, 1, 8, tp, tq, part)) return;
     a.x.rows = rows;
     const int p0 = (int)tp * S::BP, q0 = (int)tq * S::BQ;
     f32x4 acc[S::MP][S::MQ];
@@ -398,10 +398,10 @@ product_kernel(ProductArgs a)
     if (DW) a.steps = (rows + kStepK - 1) / kStepK;
     else a.q.rows = rows;
     const uint32_t tiles_p = (a.p.rows + S::BP - 1) / S::BP, tiles_q = (a.q.rows + S::BQ - 1) / S::BQ;
-    uint32_t tp, tq;
-    if (!tile_of(blockIdx.x, tiles_p, tiles_q, 8, tp, tq)) return;
+    uint32_t tp, tq, split;
+    if (!tile_of(blockIdx.x, tiles_p, tiles_q, a.splits, 8, tp, tq, split)) return;
     const int limit = DW ? a.steps * kStepK : a.limit_p;
-    const int total = a.steps * a.pairs.count, split = blockIdx.y;
+    const int total = a.steps * a.pairs.count;
     const int begin = (int)((int64_t)total * split / a.splits), end = (int)((int64_t)total * (split + 1) / a.splits);
     const int p0 = (int)tp * S::BP, q0 = (int)tq * S::BQ;
     f32x4 acc[S::MP][S::MQ];
@@ -427,9 +427,13 @@ product_kernel(ProductArgs a)
             if (p >= a.p.rows) continue;
             if (a.splits > 1) {
                 float *at = a.partial + ((int64_t)split * a.most + q) * a.p.rows + p;
+                if (a.p.rows % 4 == 0) {
+                    *reinterpret_cast<f32x4 *>(at) = acc[i][j];
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (p + e < a.p.rows) at[e] = acc[i][j][e];
+                    for (int e = 0; e < 4; e++)
+                        if (p + e < a.p.rows) at[e] = acc[i][j][e];
+                }
             } else {
                 finish(a, by, q, p, acc[i][j]);
             }
@@ -449,8 +453,12 @@ join_splits_kernel(ProductArgs a)
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s = 0; s < a.splits; s++) {
         const float *at = a.partial + ((int64_t)s * a.most + q) * a.p.rows + p;
+        if (a.p.rows % 4 == 0) {
+            v += *reinterpret_cast<const f32x4 *>(at);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] += p + e < a.p.rows ? at[e] : 0.0f;
+            for (int e = 0; e < 4; e++) v[e] += p + e < a.p.rows ? at[e] : 0.0f;
+        }
     }
     finish(a, a.head->coefficient * a.unscale, q, p, v);
 }
@@ -511,11 +519,16 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.logits_shape = shape_for(vocab, s.chunk);
     s.groups = (vocab + kShapeP[s.logits_shape] - 1) / kShapeP[s.logits_shape] * (kShapeP[s.logits_shape] / kShapeSpan[s.logits_shape]);
     if (gradients) {
+        // few outputs, a long sum: parts of it until every CU has work (two workgroups of the smaller shapes fit a CU), as
+        // long as a part is worth a tile's beginning and end
+        const int steps = s.padded / kStepK * (s.planes == 3 ? 6 : 1);
+        const auto parts = [&](int shape) {
+            const int want = (shape == kWide ? 256 : 512) / tiles(shape, dim, s.chunk), most = steps / 16;
+            return want < 1 || most < 1 ? 1 : want < most ? want : most;
+        };
         s.dx_shape = shape_for(dim, s.chunk);
-        // few outputs, a long sum: parts of it until every CU has work (two workgroups of the smaller shapes fit a CU)
-        const int tile = tiles(s.dx_shape, dim, s.chunk), want = s.dx_shape == kWide ? 256 : 512, steps = s.padded / kStepK;
-        s.dx_splits = tile >= want ? 1 : want / tile < steps / 8 ? want / tile : steps / 8;
-        if (s.dx_splits < 1) s.dx_splits = 1;
+        if (s.dx_shape == kSquare && tiles(kWide, dim, s.chunk) * parts(kWide) >= 192) s.dx_shape = kWide;
+        s.dx_splits = parts(s.dx_shape);
         s.dw_shape = shape_for(dim, vocab);
         if (s.dw_shape == kFlat) s.dw_shape = kSquare;
     }
@@ -583,7 +596,7 @@ static void launch_logits(int shape, const LogitsArgs &a, int rows, hipStream_t 
 template <typename T, bool DW>
 static void launch_product(int shape, const ProductArgs &a, int p, int q, hipStream_t stream)
 {
-    const dim3 grid((tiles(shape, p, q) + 7) / 8 * 8, a.splits);
+    const unsigned grid = ((unsigned)tiles(shape, p, q) * a.splits + 7) / 8 * 8;
     if (shape == kWide) product_kernel<T, WideShape, DW><<<grid, WideShape::THREADS, 0, stream>>>(a);
     else if (shape == kSquare) product_kernel<T, SquareShape, DW><<<grid, SquareShape::THREADS, 0, stream>>>(a);
     else if constexpr (!DW) product_kernel<T, FlatShape, DW><<<grid, FlatShape::THREADS, 0, stream>>>(a);

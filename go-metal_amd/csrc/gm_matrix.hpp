@@ -147,13 +147,17 @@ struct Tile {
     }
 };
 
-// Workgroups go round the eight XCDs, each with an L2 of its own: consecutive tiles are given to one XCD.  Within them
-// runs of `group` tiles along q share a tile of P.  false: no tile for this workgroup.
-__device__ inline bool tile_of(uint32_t block, uint32_t tiles_p, uint32_t tiles_q, uint32_t group, uint32_t &tp, uint32_t &tq)
+// Workgroups go round the eight XCDs, each with an L2 of its own: consecutive pieces of work are given to one XCD.  They are
+// the tiles of one part of the sum after those of another, and within a part runs of `group` tiles along q share a
+// tile of P.  false: nothing for this workgroup.
+__device__ inline bool tile_of(uint32_t block, uint32_t tiles_p, uint32_t tiles_q, uint32_t parts, uint32_t group, uint32_t &tp, uint32_t &tq,
+                               uint32_t &part)
 {
-    const uint32_t total = tiles_p * tiles_q, per = (total + 7) / 8;
-    const uint32_t local = block / 8, t = (block & 7) * per + local;
-    if (local >= per || t >= total) return false;
+    const uint32_t tiles = tiles_p * tiles_q, total = tiles * parts, per = (total + 7) / 8;
+    const uint32_t local = block / 8, w = (block & 7) * per + local;
+    if (local >= per || w >= total) return false;
+    part = w / tiles;
+    const uint32_t t = w - part * tiles;
     const uint32_t in_group = group * tiles_p, g = t / in_group, rest = t - g * in_group;
     const uint32_t height = tiles_q - g * group < group ? tiles_q - g * group : group;
     tp = rest / height;
@@ -255,6 +259,8 @@ __device__ inline void multiply_tiles(const Operand &p, const Operand &q, const 
         for (int j = 0; j < S::MQ; j++) acc[i][j] = multiply_add<T>(fp[i], fq[half][j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
     };
+    // Q's fragments are all needed by the next half's first row: they are read behind the first rows
+    constexpr int kEarly = S::MP >= 2 * S::MQ ? 1 : S::MP >= S::MQ ? 2 : S::MQ;
     int stage = 0;
     // `more`: a step is left to load, and all stages are under way
     const auto whole_step = [&](auto more) {
@@ -262,7 +268,7 @@ __device__ inline void multiply_tiles(const Operand &p, const Operand &q, const 
         for (int i = 0; i < S::MP; i++) {      // the first half; the second one's fragments are read
             row(0, i);
 #pragma unroll
-            for (int j = i * S::MQ / S::MP; j < (i + 1) * S::MQ / S::MP; j++) fq[1][j] = TQ::fragment(at_q, j, 1);
+            for (int j = i * kEarly; j < (i + 1) * kEarly && j < S::MQ; j++) fq[1][j] = TQ::fragment(at_q, j, 1);
             fp[i] = TP::fragment(at_p, i, 1);
         }
         const bool wraps = stage == S::STAGES - 1;
@@ -280,7 +286,7 @@ __device__ inline void multiply_tiles(const Operand &p, const Operand &q, const 
             constexpr int kRows = S::MP - kMeet;
             const int at = i - kMeet;
 #pragma unroll
-            for (int j = at * S::MQ / kRows; j < (at + 1) * S::MQ / kRows; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
+            for (int j = at * kEarly; j < (at + 1) * kEarly && j < S::MQ; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
 #pragma unroll
             for (int r = i == kMeet ? 0 : i; r <= i; r++) fp[r] = TP::fragment(at_p, r, 0);
             if constexpr (more) {
