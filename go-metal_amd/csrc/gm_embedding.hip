@@ -46,46 +46,93 @@ lookup_kernel(const T *table, const int *tokens, T *out, uint32_t rows, uint32_t
 // comparisons over the whole chip.  Longer lists are sorted in chunks; a token's place in the whole is then its
 // place in its chunk plus a binary search in every other one.
 constexpr int kSortChunk = 8192;
-constexpr int kSortRows = 32;         // tokens a workgroup places
-constexpr int kSortSlices = 32;       // parts of the chunk that its lanes compare with
+constexpr int kSortLanes = 16;        // lanes that share a part of the chunk; each compares kSortOwn tokens of its own with it
+constexpr int kSortOwn = 2;
+constexpr int kSortRows = kSortLanes * kSortOwn, kSortSlices = 64, kSortBlock = kSortLanes * kSortSlices;
+constexpr uint32_t kNoToken = 0xFFFFFFFFu;
+// Vocabularies below this fit a sort key of token and position in one 32-bit word, one comparison instead of three.
+constexpr uint32_t kShortVocab = (1u << 19) - 1;
 
-// Padding and tokens outside the vocabulary sort behind everything else.
-__device__ inline uint32_t sort_key(int token, uint32_t vocab, int padding)
+// Zeros for the table's gradient, written by the workgroups behind the sorting ones: rows that tokens name are written again
+// when they are summed (an eighth more bytes for the batches measured), and in exchange the store, which is most of a
+// gradient's time, runs while the sort computes.
+struct FillArgs {
+    char *out;
+    int64_t row_bytes, stride_bytes;
+    uint32_t rows, rows_each;       // rows of one workgroup
+};
+
+__device__ inline void fill_rows(const FillArgs &f, uint32_t block)
 {
-    return (uint32_t)token < vocab && token != padding ? (uint32_t)token : 0xFFFFFFFFu;
+    typedef uint32_t Vec __attribute__((ext_vector_type(4)));
+    const uint32_t first = block * f.rows_each, count = f.rows - first < f.rows_each ? f.rows - first : f.rows_each;
+    const bool flat = f.stride_bytes == f.row_bytes;
+    const uint32_t runs = flat ? 1 : count;
+    const int64_t bytes = flat ? f.row_bytes * count : f.row_bytes;
+    for (uint32_t r = 0; r < runs; r++) {
+        char *to = f.out + (int64_t)(first + r) * f.stride_bytes;
+        int64_t head = (int64_t)((16 - ((uintptr_t)to & 15)) & 15);
+        head = head < bytes ? head : bytes;
+        const int64_t whole = (bytes - head) / 16;
+        for (int64_t i = threadIdx.x; i < whole; i += kSortBlock) reinterpret_cast<Vec *>(to + head)[i] = Vec{0u, 0u, 0u, 0u};
+        if (threadIdx.x < 32) {         // (elements are 2 or 4 bytes: heads and tails are pairs of bytes)
+            const int64_t at = threadIdx.x < 8 ? (int64_t)threadIdx.x * 2 : head + whole * 16 + ((int64_t)threadIdx.x - 8) * 2;
+            const int64_t end = threadIdx.x < 8 ? head : bytes;
+            if (at < end) *reinterpret_cast<uint16_t *>(to + at) = 0;
+        }
+    }
 }
 
-__global__ void __launch_bounds__(kSortRows *kSortSlices)
-sort_chunk_kernel(const int *tokens, uint32_t n, uint32_t vocab, int padding, uint32_t *keys, uint32_t *positions)
+// SHORT: a key is token << 13 | position in the chunk; otherwise the token, and positions are compared where tokens are equal.
+template <bool SHORT>
+__global__ void __launch_bounds__(kSortBlock)
+sort_chunk_kernel(const int *tokens, uint32_t n, uint32_t vocab, int padding, uint32_t *keys, uint32_t *positions, uint32_t sort_blocks,
+                  FillArgs fill)
 {
-    __shared__ uint32_t all[kSortChunk];
+    if (blockIdx.x >= sort_blocks) {
+        fill_rows(fill, blockIdx.x - sort_blocks);
+        return;
+    }
+    __shared__ __attribute__((aligned(16))) uint32_t all[kSortChunk];
     __shared__ uint32_t before[kSortRows];
-    const uint32_t first = blockIdx.y * kSortChunk;
+    constexpr uint32_t kBlocks = kSortChunk / kSortRows;      // per chunk
+    const uint32_t chunk = blockIdx.x / kBlocks, first = chunk * kSortChunk, row = (blockIdx.x - chunk * kBlocks) * kSortRows;
     const uint32_t len = n - first < kSortChunk ? n - first : kSortChunk;
-    if (blockIdx.x * kSortRows >= len) return;
-    const uint32_t filled = (len + 4 * kSortSlices - 1) / (4 * kSortSlices) * (4 * kSortSlices);      // whole slices of fours
-    for (uint32_t i = threadIdx.x; i < filled; i += kSortRows * kSortSlices)
-        all[i] = i < len ? sort_key(tokens[first + i], vocab, padding) : 0xFFFFFFFFu;
+    if (row >= len) return;
+    const uint32_t filled = (len + 4 * kSortSlices - 1) / (4 * kSortSlices) * (4 * kSortSlices);      // whole rounds of fours
+    // Padding and tokens outside the vocabulary sort behind everything else; what fills the last round, behind them.
+    for (uint32_t i = threadIdx.x; i < filled; i += kSortBlock) {
+        const int t = i < len ? tokens[first + i] : -1;
+        const bool counts = (uint32_t)t < vocab && t != padding;
+        all[i] = SHORT ? (i < len ? (counts ? (uint32_t)t : kShortVocab) << 13 | i : kNoToken) : counts ? (uint32_t)t : kNoToken;
+    }
     if (threadIdx.x < kSortRows) before[threadIdx.x] = 0;
     __syncthreads();
-    const uint32_t r = threadIdx.x % kSortRows, slice = threadIdx.x / kSortRows;
-    const uint32_t mine = blockIdx.x * kSortRows + r;
-    const uint32_t key = mine < len ? all[mine] : 0xFFFFFFFFu;
-    const uint32_t per = filled / kSortSlices;
-    uint32_t count = 0;
-    for (uint32_t j = slice * per; j < (slice + 1) * per; j += 4) {
-        const uint4 k = *reinterpret_cast<const uint4 *>(&all[j]);
-        // (the filling behind the list has the largest key and later positions: it is never before anything)
-        count += (k.x < key) | ((k.x == key) & (j < mine));
-        count += (k.y < key) | ((k.y == key) & (j + 1 < mine));
-        count += (k.z < key) | ((k.z == key) & (j + 2 < mine));
-        count += (k.w < key) | ((k.w == key) & (j + 3 < mine));
+    const uint32_t lane = threadIdx.x % kSortLanes, slice = threadIdx.x / kSortLanes;
+    uint32_t mine[kSortOwn], key[kSortOwn], count[kSortOwn];
+#pragma unroll
+    for (int o = 0; o < kSortOwn; o++) {
+        mine[o] = row + o * kSortLanes + lane;
+        key[o] = mine[o] < len ? all[mine[o]] : kNoToken;
+        count[o] = 0;
     }
-    atomicAdd(&before[r], count);      // whole numbers: their order does not matter
+    for (uint32_t j = slice * 4; j < filled; j += 4 * kSortSlices) {      // (a wavefront's four parts lie side by side)
+        const uint4 k4 = *reinterpret_cast<const uint4 *>(&all[j]);
+        const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+        for (int o = 0; o < kSortOwn; o++)
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++)
+                count[o] += SHORT ? k[c] < key[o] : (uint32_t)((k[c] < key[o]) | ((k[c] == key[o]) & (j + c < mine[o])));
+    }
+#pragma unroll
+    for (int o = 0; o < kSortOwn; o++) atomicAdd(&before[o * kSortLanes + lane], count[o]);      // whole numbers: their order does not matter
     __syncthreads();
-    if (threadIdx.x < kSortRows && mine < len) {
-        keys[first + before[r]] = key;
-        positions[first + before[r]] = first + mine;
+    const uint32_t me = row + threadIdx.x;
+    if (threadIdx.x < kSortRows && me < len) {
+        const uint32_t token = SHORT ? all[me] >> 13 : all[me];
+        keys[first + before[threadIdx.x]] = SHORT && token == kShortVocab ? kNoToken : token;
+        positions[first + before[threadIdx.x]] = first + me;
     }
 }
 
@@ -119,12 +166,18 @@ merge_chunks_kernel(const uint32_t *keys, const uint32_t *positions, uint32_t n,
 }
 
 // ------------------------------------------------------------------------------------------ summing the runs ----
-// The sorted list is cut into pieces of kPiece entries, so that a token that fills a tenth of a batch is summed by
+// The sorted list is cut into pieces of 8 to 32 entries, so that a token that fills a tenth of a batch is summed by
 // many workgroups.  A run that lies in one piece goes straight to its row; of one that crosses a border every piece
 // leaves a partial sum (slot 0: the run the piece begins in the middle of; slot 1: the run it ends in the middle
 // of), which join_runs_kernel adds up in the pieces' order.
-constexpr int kPiece = 32;
 constexpr int kSumBlock = 64;              // one wavefront, eight elements a lane
+
+// Long pieces leave fewer partial sums, short ones more wavefronts: the longest that leave four for each SIMD.
+static uint32_t piece_for(size_t n, size_t dim)
+{
+    const size_t tiles = (dim + kSumBlock * 8 - 1) / (kSumBlock * 8);
+    return n * tiles >= 4096 * 32 ? 32 : n * tiles >= 4096 * 16 ? 16 : 8;
+}
 
 struct SumArgs {
     const uint32_t *keys, *positions;
@@ -135,7 +188,7 @@ struct SumArgs {
     float *partial;                        // [piece][2][dim]
     DropoutParams d;
     bool in_aligned, out_aligned;
-    uint32_t col_tiles, sum_blocks;
+    uint32_t col_tiles, piece;
 };
 
 template <typename O>
@@ -156,35 +209,13 @@ __device__ inline void write_row(O *out, const SumArgs &a, uint32_t row, uint32_
     store8(p, whole, count, v);
 }
 
-// Workgroups below sum_blocks sum a piece's columns; the others write zeros to the rows that no token names (there
-// are none of those when the gradient is added to what is there).
 template <typename T, typename O>
 __global__ void __launch_bounds__(kSumBlock)
 sum_runs_kernel(const T *dy, O *out, SumArgs a)
 {
-    if (blockIdx.x >= a.sum_blocks) {
-        // 64 rows a workgroup: a lane looks one of them up, then the wavefront fills the absent ones together
-        const uint32_t row = (blockIdx.x - a.sum_blocks) * 64 + threadIdx.x;
-        bool absent = row < a.vocab;
-        if (absent) {
-            const uint32_t at = keys_before(a.keys, a.n, row, false);
-            absent = at >= a.n || a.keys[at] != row;
-        }
-        uint64_t todo = __ballot(absent);
-        const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        while (todo) {
-            const uint32_t r = row - threadIdx.x + (uint32_t)__builtin_ctzll(todo);
-            todo &= todo - 1;
-            for (uint32_t col = threadIdx.x * 8; col < a.dim; col += kSumBlock * 8) {
-                const int count = a.dim - col < 8 ? (int)(a.dim - col) : 8;
-                store8(out + (int64_t)r * a.out_stride + col, a.out_aligned && count == 8, count, zero);
-            }
-        }
-        return;
-    }
     const uint32_t piece = blockIdx.x / a.col_tiles;
     const uint32_t col = (blockIdx.x - piece * a.col_tiles) * (kSumBlock * 8) + threadIdx.x * 8;
-    const uint32_t lo = piece * kPiece, hi = a.n - lo < kPiece ? a.n : lo + kPiece;
+    const uint32_t lo = piece * a.piece, hi = a.n - lo < a.piece ? a.n : lo + a.piece;
     // the piece's entries, one a lane: later every lane takes them from there
     const uint32_t l = threadIdx.x;
     const uint32_t my_key = lo + l < hi ? a.keys[lo + l] : 0xFFFFFFFFu;
@@ -200,7 +231,7 @@ sum_runs_kernel(const T *dy, O *out, SumArgs a)
     if (a.d.state) st = *a.d.state;
     float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     bool from_before = __builtin_amdgcn_readlane(my_key, 0) == key_before;
-    constexpr uint32_t kAhead = 4;         // rows in flight a lane
+    constexpr uint32_t kAhead = sizeof(T) == 2 ? 8 : 4;         // rows in flight a lane
     for (uint32_t i = 0; i < entries; i += kAhead) {
         float v[kAhead][8];
 #pragma unroll
@@ -239,23 +270,29 @@ join_runs_kernel(O *out, SumArgs a)
 {
     const uint32_t piece = blockIdx.x / a.col_tiles;
     const uint32_t col = (blockIdx.x - piece * a.col_tiles) * (kSumBlock * 8) + threadIdx.x * 8;
-    const uint32_t border = (piece + 1) * kPiece;      // (the grid leaves the last piece out: border < n)
+    const uint32_t border = (piece + 1) * a.piece;      // (the grid leaves the last piece out: border < n)
     const uint32_t key = a.keys[border - 1];
     if (key == 0xFFFFFFFFu || a.keys[border] != key) return;
-    const uint32_t lo = piece * kPiece;
+    const uint32_t lo = piece * a.piece;
     if (lo > 0 && a.keys[lo - 1] == key) return;       // it began in an earlier piece
     if (col >= a.dim) return;
     const uint32_t end = border + keys_before(a.keys + border, a.n - border, key, true);
-    const uint32_t last = (end - 1) / kPiece;
+    const uint32_t last = (end - 1) / a.piece;
     const int count = a.dim - col < 8 ? (int)(a.dim - col) : 8;
     const bool whole = count == 8 && a.dim % 4 == 0;
     float acc[8];
     load8(a.partial + ((int64_t)piece * 2 + 1) * a.dim + col, whole, count, acc);
-    for (uint32_t c = piece + 1; c <= last; c++) {
-        float v[8];
-        load8(a.partial + (int64_t)c * 2 * a.dim + col, whole, count, v);
+    constexpr uint32_t kAhead = 8;      // partial sums in flight a lane (a word that fills a tenth of a batch has a hundred)
+    for (uint32_t c = piece + 1; c <= last; c += kAhead) {
+        float v[kAhead][8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) acc[e] = acc[e] + v[e];
+        for (uint32_t k = 0; k < kAhead; k++) load8(a.partial + (int64_t)(c + k <= last ? c + k : last) * 2 * a.dim + col, whole, count, v[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++)
+            if (c + k <= last) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) acc[e] = acc[e] + v[k][e];
+            }
     }
     write_row(out, a, key, col, acc);
 }
@@ -274,7 +311,8 @@ static GradientSpace gradient_space(size_t n, size_t dim)
     s.positions = at, at += up(4 * n);
     s.chunk_keys = at, at += n > kSortChunk ? up(4 * n) : 0;
     s.chunk_positions = at, at += n > kSortChunk ? up(4 * n) : 0;
-    s.partial = at, at += n > kPiece ? up((n + kPiece - 1) / kPiece * 2 * dim * 4) : 0;
+    const size_t piece = piece_for(n, dim);
+    s.partial = at, at += n > piece ? up((n + piece - 1) / piece * 2 * dim * 4) : 0;
     s.bytes = at;
     return s;
 }
@@ -390,9 +428,15 @@ try {
     const uint32_t n = (uint32_t)num_tokens;
     SumArgs a{};
     a.col_tiles = ((uint32_t)dim + kSumBlock * 8 - 1) / (kSumBlock * 8);
-    const uint64_t pieces = ((uint64_t)n + kPiece - 1) / kPiece;
-    const uint64_t fill = accumulate ? 0 : ((uint64_t)vocab_size + 63) / 64;
-    if (pieces * a.col_tiles + fill > 0x7FFFFFFFull || ((uint64_t)n + kSortChunk - 1) / kSortChunk > 65535) {
+    a.piece = piece_for(n, (size_t)dim);
+    const uint64_t pieces = ((uint64_t)n + a.piece - 1) / a.piece;
+    // a filling workgroup takes rows of 16 KiB together: a store a lane
+    FillArgs fill{reinterpret_cast<char *>(table_gradient_buffer), (int64_t)dim * (int64_t)out, (int64_t)table_gradient_stride * (int64_t)out,
+                  (uint32_t)vocab_size, 1};
+    fill.rows_each = fill.row_bytes < 16384 ? (uint32_t)(16384 / fill.row_bytes) : 1;
+    const uint64_t fills = accumulate ? 0 : ((uint64_t)vocab_size + fill.rows_each - 1) / fill.rows_each;
+    const uint64_t sorts = ((uint64_t)n + kSortChunk - 1) / kSortChunk * (kSortChunk / kSortRows);
+    if (pieces * a.col_tiles > 0x7FFFFFFFull || sorts + fills > 0x7FFFFFFFull) {
         set_error("a gradient of %d rows of %d elements needs more workgroups than one launch can address", num_tokens, dim);
         return kRcRange;
     }
@@ -404,16 +448,17 @@ try {
     if (!scope.ok()) return kRcHip;
     uint32_t *keys = reinterpret_cast<uint32_t *>(workspace + space.keys);
     uint32_t *positions = reinterpret_cast<uint32_t *>(workspace + space.positions);
-    if (n > 0) {
-        const bool chunks = n > kSortChunk;
-        uint32_t *to_keys = chunks ? reinterpret_cast<uint32_t *>(workspace + space.chunk_keys) : keys;
-        uint32_t *to_positions = chunks ? reinterpret_cast<uint32_t *>(workspace + space.chunk_positions) : positions;
-        const uint32_t longest = chunks ? kSortChunk : n;
-        const dim3 grid((longest + kSortRows - 1) / kSortRows, (n + kSortChunk - 1) / kSortChunk);
-        sort_chunk_kernel<<<grid, kSortRows * kSortSlices, 0, stream>>>(reinterpret_cast<const int *>(token_buffer), n,
-                                                                        (uint32_t)vocab_size, padding_token, to_keys, to_positions);
-        if (chunks) merge_chunks_kernel<<<(n + 255) / 256, 256, 0, stream>>>(to_keys, to_positions, n, keys, positions);
+    const bool chunks = n > kSortChunk;
+    uint32_t *to_keys = chunks ? reinterpret_cast<uint32_t *>(workspace + space.chunk_keys) : keys;
+    uint32_t *to_positions = chunks ? reinterpret_cast<uint32_t *>(workspace + space.chunk_positions) : positions;
+    // (of a list shorter than a chunk only the workgroups that have rows to place are launched)
+    const uint32_t sort_blocks = chunks ? (uint32_t)sorts : (n + kSortRows - 1) / kSortRows;
+    if (sort_blocks + fills > 0) {
+        const auto sort = (uint32_t)vocab_size < kShortVocab ? sort_chunk_kernel<true> : sort_chunk_kernel<false>;
+        sort<<<sort_blocks + (uint32_t)fills, kSortBlock, 0, stream>>>(reinterpret_cast<const int *>(token_buffer), n, (uint32_t)vocab_size,
+                                                                       padding_token, to_keys, to_positions, sort_blocks, fill);
     }
+    if (chunks) merge_chunks_kernel<<<(n + 255) / 256, 256, 0, stream>>>(to_keys, to_positions, n, keys, positions);
     a.keys = keys;
     a.positions = positions;
     a.n = n;
@@ -427,8 +472,7 @@ try {
     a.d = d;
     a.in_aligned = output_gradient_buffer % 16 == 0 && (size_t)output_gradient_stride * in % 16 == 0;
     a.out_aligned = table_gradient_buffer % 16 == 0 && (size_t)table_gradient_stride * out % 16 == 0;
-    a.sum_blocks = (uint32_t)(pieces * a.col_tiles);
-    const uint32_t grid = a.sum_blocks + (uint32_t)fill, join_grid = pieces > 1 ? (uint32_t)(pieces - 1) * a.col_tiles : 0;
+    const uint32_t grid = (uint32_t)(pieces * a.col_tiles), join_grid = pieces > 1 ? (uint32_t)(pieces - 1) * a.col_tiles : 0;
     const auto launch = data_type == kFloat32                                       ? launch_sums<float, float>
                         : data_type == kFloat16 && gradient_type == kFloat16        ? launch_sums<_Float16, _Float16>
                         : data_type == kFloat16                                     ? launch_sums<_Float16, float>
