@@ -175,6 +175,9 @@ logits_kernel(LogitsArgs a)
     const int wp = p0 + wave / S::WQ * (S::BP / S::WP) + (lane >> 4) * 4, wq = q0 + wave % S::WQ * (S::BQ / S::WQ) + (lane & 15);
     const int group = (p0 + wave / S::WQ * (S::BP / S::WP)) / (S::BP / S::WP);
     const bool ragged = p0 + S::BP > a.vocab;
+    const uint32_t lds = (uint32_t)(uintptr_t)(GM_LDS char *)tiles;
+    const int wave_p = wp - (lane >> 4) * 4, wave_q = wq - (lane & 15);
+    __builtin_amdgcn_s_barrier();      // the tiles' memory turns rows from here on
 #pragma unroll
     for (int j = 0; j < S::MQ; j++) {
         const int q = wq + j * 16;
@@ -202,32 +205,28 @@ logits_kernel(LogitsArgs a)
         top = fmaxf(top, __shfl_xor(top, 32));
         const float ref = top == -INFINITY ? 0.0f : top;      // (a share that lies behind the vocabulary: all zeros)
         float sum = 0.0f;
-        const int64_t row = q * a.stride;
+        f32x4 v[S::MP];
         if (a.keep == kKeepFloat) {
 #pragma unroll
-            for (int i = 0; i < S::MP; i++) {
-                f32x4 e;
+            for (int i = 0; i < S::MP; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) sum += e[r] = expf(acc[i][j][r] - ref);
-                if (there && wp + i * 16 < a.padded) *reinterpret_cast<f32x4 *>(static_cast<float *>(a.kept) + row + wp + i * 16) = e;
-            }
+                for (int r = 0; r < 4; r++) sum += v[i][r] = expf(acc[i][j][r] - ref);
         } else {
             // 2^15 exp(s - ref) by the hardware's power of two; the sum's factor is taken out again exactly
-            typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-            for (int i = 0; i < S::MP; i++) {
-                f16x4 h;
+            for (int i = 0; i < S::MP; i++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r] - ref, 1.44269504f, kExpShift));
-                    sum += e;
-                    h[r] = (_Float16)e;
-                }
-                if (a.keep == kKeepHalf && there && wp + i * 16 < a.padded)
-                    *reinterpret_cast<f16x4 *>(static_cast<_Float16 *>(a.kept) + row + wp + i * 16) = h;
-            }
+                for (int r = 0; r < 4; r++) sum += v[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r] - ref, 1.44269504f, kExpShift));
             sum *= 1.0f / kExpScale;
         }
+        if (a.keep != kKeepNothing)
+            turn_rows<S>(lds, v, [&](int row, int p, const float (&e)[8]) {
+                const int to = wave_q + j * 16 + row, col = wave_p + p;
+                if (to >= rows || col >= a.padded) return;
+                const int64_t at = to * a.stride + col;
+                if (a.keep == kKeepFloat) store8(static_cast<float *>(a.kept) + at, true, 8, e);
+                else store8(static_cast<_Float16 *>(a.kept) + at, true, 8, e);
+            });
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         if (there && lane < 16) a.stats[(int64_t)q * a.groups + group] = float2{top, sum};
@@ -346,45 +345,41 @@ struct ProductArgs {
     int out_type;
     int accumulate;                  // add what `out` holds
     const float *add;                // and this, of out's shape without gaps (nullptr: nothing)
-    bool out_aligned;                // rows of out begin at multiples of four elements
+    bool out_aligned;                // rows of out begin at multiples of 16 bytes
     bool skip_empty;                 // a chunk without tokens leaves `out` alone
 };
 
 template <typename O>
-__device__ inline void finish4(const ProductArgs &a, O *out, int64_t row, int p, f32x4 v)
+__device__ inline void finish_as(const ProductArgs &a, O *out, int64_t row, int p, float (&v)[8])
 {
-    typedef O Vec __attribute__((ext_vector_type(4)));
-    const int count = a.p.rows - p < 4 ? a.p.rows - p : 4;
+    const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
+    const bool whole = a.out_aligned && count == 8;
     O *at = out + row * a.out_stride + p;
-    if (a.out_aligned && count == 4) {
-        Vec o;
-        if (a.accumulate) {
-            o = *reinterpret_cast<const Vec *>(at);
+    if (a.accumulate) {
+        float old[8];
+        load8(at, whole, count, old);
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = (float)o[e] + v[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = from_float<O>(v[e]);
-        *reinterpret_cast<Vec *>(at) = o;
-        return;
+        for (int e = 0; e < 8; e++) v[e] = old[e] + v[e];
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (e < count) at[e] = from_float<O>(a.accumulate ? (float)at[e] + v[e] : v[e]);
+    store8(at, whole, count, v);
 }
 
-// Four outputs of one row: times c, added to what is there, rounded once.
-__device__ inline void finish(const ProductArgs &a, float by, int q, int p, f32x4 v)
+// Eight outputs of one row: times c, added to what is there, rounded once.
+__device__ inline void finish(const ProductArgs &a, float by, int q, int p, float (&v)[8])
 {
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = v[e] * by;
-    if (a.add)
+    for (int e = 0; e < 8; e++) v[e] = v[e] * by;
+    if (a.add) {
+        const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
+        float more[8];
+        load8(a.add + (int64_t)q * a.p.rows + p, count == 8 && a.p.rows % 4 == 0, count, more);
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = p + e < a.p.rows ? a.add[(int64_t)q * a.p.rows + p + e] + v[e] : 0.0f;
+        for (int e = 0; e < 8; e++) v[e] = more[e] + v[e];
+    }
     const int64_t row = a.row_of ? a.row_of[a.first + q] : q;
-    if (a.out_type == kFloat32) finish4(a, static_cast<float *>(a.out), row, p, v);
-    else if (a.out_type == kFloat16) finish4(a, static_cast<_Float16 *>(a.out), row, p, v);
-    else finish4(a, static_cast<__bf16 *>(a.out), row, p, v);
+    if (a.out_type == kFloat32) finish_as(a, static_cast<float *>(a.out), row, p, v);
+    else if (a.out_type == kFloat16) finish_as(a, static_cast<_Float16 *>(a.out), row, p, v);
+    else finish_as(a, static_cast<__bf16 *>(a.out), row, p, v);
 }
 
 // DW: Q is dS across and the sum runs over the chunk's tokens; otherwise dX, Q is dS along.  P lies across in both.
@@ -415,52 +410,54 @@ product_kernel(ProductArgs a)
             for (int j = 0; j < S::MQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const float by = a.head->coefficient * a.unscale;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wp = p0 + wave / S::WQ * (S::BP / S::WP) + (lane >> 4) * 4, wq = q0 + wave % S::WQ * (S::BQ / S::WQ) + (lane & 15);
+    const int wave = threadIdx.x >> 6;
+    const int wave_p = p0 + wave / S::WQ * (S::BP / S::WP), wave_q = q0 + wave % S::WQ * (S::BQ / S::WQ);
+    __builtin_amdgcn_s_barrier();      // the tiles' memory turns rows from here on
 #pragma unroll
     for (int j = 0; j < S::MQ; j++) {
-        const int q = wq + j * 16;
-        if (q >= a.q.rows) continue;
+        if (wave_q + j * 16 >= a.q.rows) break;
+        f32x4 v[S::MP];
 #pragma unroll
-        for (int i = 0; i < S::MP; i++) {
-            const int p = wp + i * 16;
-            if (p >= a.p.rows) continue;
+        for (int i = 0; i < S::MP; i++) v[i] = acc[i][j];
+        turn_rows<S>((uint32_t)(uintptr_t)(GM_LDS char *)tiles, v, [&](int row, int p, float (&out)[8]) {
+            const int q = wave_q + j * 16 + row;
+            p += wave_p;
+            if (q >= a.q.rows || p >= a.p.rows) return;
             if (a.splits > 1) {
-                float *at = a.partial + ((int64_t)split * a.most + q) * a.p.rows + p;
-                if (a.p.rows % 4 == 0) {
-                    *reinterpret_cast<f32x4 *>(at) = acc[i][j];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (p + e < a.p.rows) at[e] = acc[i][j][e];
-                }
+                const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
+                store8(a.partial + ((int64_t)split * a.most + q) * a.p.rows + p, count == 8 && a.p.rows % 4 == 0, count, out);
             } else {
-                finish(a, by, q, p, acc[i][j]);
+                finish(a, by, q, p, out);
             }
-        }
+        });
     }
 }
 
-// The parts of a split sum, added up in order; four outputs a lane.
+// The parts of a split sum, added up in order; eight outputs a lane.
 __global__ void __launch_bounds__(256)
 join_splits_kernel(ProductArgs a)
 {
     const int rows = chunk_rows(a.head, a.first, a.most);
-    const int per_row = (a.p.rows + 3) / 4;
+    const int per_row = (a.p.rows + 7) / 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int q = (int)(i / per_row), p = (int)(i - (int64_t)q * per_row) * 4;
+    const int q = (int)(i / per_row), p = (int)(i - (int64_t)q * per_row) * 8;
     if (q >= rows) return;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; s++) {
-        const float *at = a.partial + ((int64_t)s * a.most + q) * a.p.rows + p;
-        if (a.p.rows % 4 == 0) {
-            v += *reinterpret_cast<const f32x4 *>(at);
-        } else {
+    const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
+    const bool whole = count == 8 && a.p.rows % 4 == 0;
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kAhead = 4;
+    for (int s = 0; s < a.splits; s += kAhead) {
+        float v[kAhead][8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] += p + e < a.p.rows ? at[e] : 0.0f;
-        }
+        for (int k = 0; k < kAhead; k++) load8(a.partial + ((int64_t)(s + k < a.splits ? s + k : s) * a.most + q) * a.p.rows + p, whole, count, v[k]);
+#pragma unroll
+        for (int k = 0; k < kAhead; k++)
+            if (s + k < a.splits) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum[e] += v[k][e];
+            }
     }
-    finish(a, a.head->coefficient * a.unscale, q, p, v);
+    finish(a, a.head->coefficient * a.unscale, q, p, sum);
 }
 
 // ------------------------------------------------------------------------------------------------ host side ----
@@ -651,10 +648,10 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
             a.splits = s.dx_splits, a.partial = reinterpret_cast<float *>(space + s.partial);
             a.head = head, a.row_of = row_of, a.unscale = 1.0f / kSlopeScale<T>;
             a.out = reinterpret_cast<void *>(c.dx), a.out_stride = c.dx_stride, a.out_type = c.data_type;
-            a.out_aligned = c.dx % (4 * sizeof(I)) == 0 && c.dx_stride % 4 == 0;
+            a.out_aligned = c.dx % 16 == 0 && c.dx_stride * sizeof(I) % 16 == 0;
             launch_product<T, false>(s.dx_shape, a, s.dim, tokens, stream);
             if (s.dx_splits > 1)
-                join_splits_kernel<<<(unsigned)(((int64_t)tokens * ((s.dim + 3) / 4) + 255) / 256), 256, 0, stream>>>(a);
+                join_splits_kernel<<<(unsigned)(((int64_t)tokens * ((s.dim + 7) / 8) + 255) / 256), 256, 0, stream>>>(a);
         }
         if (c.dw) {
             ProductArgs a{};
@@ -668,7 +665,7 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
                 a.out_aligned = s.dim % 4 == 0;
             } else {
                 a.out = reinterpret_cast<void *>(c.dw), a.out_stride = c.dw_stride, a.out_type = c.gradient_type;
-                a.out_aligned = c.dw % (4 * type_bytes(c.gradient_type)) == 0 && c.dw_stride % 4 == 0;
+                a.out_aligned = c.dw % 16 == 0 && c.dw_stride * type_bytes(c.gradient_type) % 16 == 0;
                 a.accumulate = c.accumulate || (k > 0 && !s.sum_weights);
                 a.add = s.sum_weights && k > 0 ? sums : nullptr;
             }

@@ -307,4 +307,29 @@ __device__ inline void multiply_tiles(const Operand &p, const Operand &q, const 
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 
+// Sixteen rows of Q's outputs go through the wavefront's own share of LDS on their way out: a lane holds four p of one q,
+// and what it would store is 8 bytes of each of sixteen rows; turned, a wavefront stores whole rows of its p, 16 bytes a
+// lane.  `use(row, p, v)` gets eight consecutive p (from the wavefront's first) of row 0 .. 15.  Every wavefront of the
+// workgroup must be done with the tiles in LDS.
+template <typename S, typename F>
+__device__ inline void turn_rows(uint32_t lds, const f32x4 (&v)[S::MP], F &&use)
+{
+    constexpr int kSpan = S::BP / S::WP, kPitch = kSpan * 4 + 16, kLanes = kSpan / 8, kRows = 64 / kLanes;
+    static_assert(S::WAVES * 16 * kPitch <= S::LDS, "room for every wavefront");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t mine = lds + wave * (16 * kPitch);
+#pragma unroll
+    for (int i = 0; i < S::MP; i++) *reinterpret_cast<GM_LDS f32x4 *>(mine + (lane & 15) * kPitch + (i * 16 + (lane >> 4) * 4) * 4) = v[i];
+#pragma unroll
+    for (int pass = 0; pass < 16 / kRows; pass++) {
+        const int row = pass * kRows + lane / kLanes, p = lane % kLanes * 8;
+        const GM_LDS f32x4 *at = reinterpret_cast<const GM_LDS f32x4 *>(mine + row * kPitch + p * 4);
+        const f32x4 a = at[0], b = at[1];
+        float out[8];
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e] = a[e], out[4 + e] = b[e];
+        use(row, p, out);
+    }
+}
+
 }  // namespace gm
