@@ -29,9 +29,10 @@ struct LossHead {
 
 typedef Shape<256, 256, 2, 4, 2> WideShape;       // products of many tiles: 128 KiB of LDS, one workgroup a CU
 typedef Shape<128, 128, 2, 2, 2> SquareShape;     // fewer tiles than a wide shape needs to fill the chip
+typedef Shape<256, 128, 4, 2, 3> TallShape;       // up to 128 tokens: the weights' stream bounds it, three steps of it in flight
 typedef Shape<128, 32, 4, 1, 4> FlatShape;        // up to 32 tokens: the weights' stream is all there is
-enum : int { kWide, kSquare, kFlat };
-constexpr int kShapeP[3] = {256, 128, 128}, kShapeQ[3] = {256, 128, 32}, kShapeSpan[3] = {128, 64, 32};
+enum : int { kWide, kSquare, kTall, kFlat };
+constexpr int kShapeP[4] = {256, 128, 256, 128}, kShapeQ[4] = {256, 128, 128, 32}, kShapeSpan[4] = {128, 64, 64, 32};
 
 // exp(s - m) in 16 bits is 32768 times itself in fp16, dS of fp16 operands 16384 times itself: both keep clear of the
 // subnormals (down to 2^-29 and 2^-28), and an entry's rounding is 2^-12 of it.
@@ -169,15 +170,20 @@ logits_kernel(LogitsArgs a)
     a.x.rows = rows;
     const int p0 = (int)tp * S::BP, q0 = (int)tq * S::BQ;
     f32x4 acc[S::MP][S::MQ];
-    multiply_tiles<T, S, false, false>(a.w, a.x, a.pairs, p0, q0, a.steps, 0, 0, 0, a.steps * a.pairs.count,
-                                       (uint32_t)(uintptr_t)(GM_LDS char *)tiles, acc);
+    const uint32_t lds = (uint32_t)(uintptr_t)(GM_LDS char *)tiles;
+    // One tile of tokens: nobody shares the weights' rows, and every workgroup begins at a k of its own.  At one k the rows of all
+    // tiles, a power of two apart, lie on one channel: 1.07 GB of weights pass at 6.2 TB/s instead of 5.
+    const int first = rows <= S::BQ && S::BQ > 32 ? (int)(tp * 5 % (uint32_t)a.steps) : 0;
+    Multiplier<T, S, false, false> product(a.w, a.x, a.pairs, a.steps, 0, 0, first, first + a.steps * a.pairs.count, lds);
+    product.start(p0, q0);
+    product.run(acc);      // (from here on the stages' memory turns rows)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wp = p0 + wave / S::WQ * (S::BP / S::WP) + (lane >> 4) * 4, wq = q0 + wave % S::WQ * (S::BQ / S::WQ) + (lane & 15);
     const int group = (p0 + wave / S::WQ * (S::BP / S::WP)) / (S::BP / S::WP);
     const bool ragged = p0 + S::BP > a.vocab;
-    const uint32_t lds = (uint32_t)(uintptr_t)(GM_LDS char *)tiles;
-    const int wave_p = wp - (lane >> 4) * 4, wave_q = wq - (lane & 15);
-    __builtin_amdgcn_s_barrier();      // the tiles' memory turns rows from here on
+    // what this lane stores of the exponentials: always the same eight words
+    const int wave_q = wq - (lane & 15), turn_col = wp - (lane >> 4) * 4 + lane % (64 / kTurnRows<S>) * 8;
+    char *kept = static_cast<char *>(a.kept) + (wave_q * a.stride + turn_col) * (a.keep == kKeepFloat ? 4 : 2);
 #pragma unroll
     for (int j = 0; j < S::MQ; j++) {
         const int q = wq + j * 16;
@@ -220,12 +226,11 @@ logits_kernel(LogitsArgs a)
             sum *= 1.0f / kExpScale;
         }
         if (a.keep != kKeepNothing)
-            turn_rows<S>(lds, v, [&](int row, int p, const float (&e)[8]) {
-                const int to = wave_q + j * 16 + row, col = wave_p + p;
-                if (to >= rows || col >= a.padded) return;
-                const int64_t at = to * a.stride + col;
-                if (a.keep == kKeepFloat) store8(static_cast<float *>(a.kept) + at, true, 8, e);
-                else store8(static_cast<_Float16 *>(a.kept) + at, true, 8, e);
+            turn_rows<S>(product.turn_place(), v, [&](int row, int, const float (&e)[8]) {
+                const int to = j * 16 + row;
+                if (turn_col >= a.padded || wave_q + to >= rows) return;
+                if (a.keep == kKeepFloat) store8(reinterpret_cast<float *>(kept) + to * a.stride, true, 8, e);
+                else store8(reinterpret_cast<_Float16 *>(kept) + to * a.stride, true, 8, e);
             });
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
@@ -382,6 +387,67 @@ __device__ inline void finish(const ProductArgs &a, float by, int q, int p, floa
     else finish_as(a, static_cast<__bf16 *>(a.out), row, p, v);
 }
 
+// The wavefront's outputs, all of which exist, to rows that begin at multiples of 16 bytes: nothing is left of finish() but
+// the product and the rounding.  (With its cases the stores of a tile took more time than 128 tokens' matrix work.)
+template <typename S, typename O>
+__device__ inline void store_whole(O *out, int64_t stride, float by, uint32_t turn, const f32x4 (&acc)[S::MP][S::MQ])
+{
+    const int lane = threadIdx.x & 63;
+    constexpr int kLanes = 64 / kTurnRows<S>;
+    O *at = out + (lane / kLanes) * stride + lane % kLanes * 8;
+#pragma unroll
+    for (int j = 0; j < S::MQ; j++) {
+        f32x4 v[S::MP];
+#pragma unroll
+        for (int i = 0; i < S::MP; i++) v[i] = acc[i][j];
+        turn_rows<S>(turn, v, [&](int, int, float (&o)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = o[e] * by;
+            store8(at, true, 8, o);
+            at += kTurnRows<S> * stride;
+        });
+    }
+}
+
+// The tile at (p0, q0) out of the workgroup's accumulators.
+template <typename S>
+__device__ inline void store_tile(const ProductArgs &a, float by, int p0, int q0, uint32_t split, uint32_t turn, const f32x4 (&acc)[S::MP][S::MQ])
+{
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_p = p0 + wave / S::WQ * (S::BP / S::WP), wave_q = q0 + wave % S::WQ * (S::BQ / S::WQ);
+    if (wave_p + S::BP / S::WP <= a.p.rows && wave_q + S::BQ / S::WQ <= a.q.rows) {
+        if (a.splits > 1 && a.p.rows % 4 == 0) {
+            store_whole<S>(a.partial + ((int64_t)split * a.most + wave_q) * a.p.rows + wave_p, a.p.rows, 1.0f, turn, acc);
+            return;
+        }
+        if (a.splits == 1 && a.out_aligned && !a.accumulate && !a.add && !a.row_of) {
+            const int64_t at = wave_q * a.out_stride + wave_p;
+            if (a.out_type == kFloat32) store_whole<S>(static_cast<float *>(a.out) + at, a.out_stride, by, turn, acc);
+            else if (a.out_type == kFloat16) store_whole<S>(static_cast<_Float16 *>(a.out) + at, a.out_stride, by, turn, acc);
+            else store_whole<S>(static_cast<__bf16 *>(a.out) + at, a.out_stride, by, turn, acc);
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < S::MQ; j++) {
+        if (wave_q + j * 16 >= a.q.rows) break;
+        f32x4 v[S::MP];
+#pragma unroll
+        for (int i = 0; i < S::MP; i++) v[i] = acc[i][j];
+        turn_rows<S>(turn, v, [&](int row, int p, float (&out)[8]) {
+            const int q = wave_q + j * 16 + row;
+            p += wave_p;
+            if (q >= a.q.rows || p >= a.p.rows) return;
+            if (a.splits > 1) {
+                const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
+                store8(a.partial + ((int64_t)split * a.most + q) * a.p.rows + p, count == 8 && a.p.rows % 4 == 0, count, out);
+            } else {
+                finish(a, by, q, p, out);
+            }
+        });
+    }
+}
+
 // DW: Q is dS across and the sum runs over the chunk's tokens; otherwise dX, Q is dS along.  P lies across in both.
 template <typename T, typename S, bool DW>
 __global__ void __launch_bounds__(S::THREADS)
@@ -399,38 +465,18 @@ product_kernel(ProductArgs a)
     const int total = a.steps * a.pairs.count;
     const int begin = (int)((int64_t)total * split / a.splits), end = (int)((int64_t)total * (split + 1) / a.splits);
     const int p0 = (int)tp * S::BP, q0 = (int)tq * S::BQ;
+    Multiplier<T, S, true, DW> product(a.p, a.q, a.pairs, a.steps, limit, limit, begin, end, (uint32_t)(uintptr_t)(GM_LDS char *)tiles);
     f32x4 acc[S::MP][S::MQ];
     if (begin < end) {
-        multiply_tiles<T, S, true, DW>(a.p, a.q, a.pairs, p0, q0, a.steps, limit, limit, begin, end,
-                                       (uint32_t)(uintptr_t)(GM_LDS char *)tiles, acc);
-    } else {
+        product.start(p0, q0);
+        product.run(acc);
+    } else {      // a chunk without tokens that dW has to be written for all the same
 #pragma unroll
         for (int i = 0; i < S::MP; i++)
 #pragma unroll
             for (int j = 0; j < S::MQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const float by = a.head->coefficient * a.unscale;
-    const int wave = threadIdx.x >> 6;
-    const int wave_p = p0 + wave / S::WQ * (S::BP / S::WP), wave_q = q0 + wave % S::WQ * (S::BQ / S::WQ);
-    __builtin_amdgcn_s_barrier();      // the tiles' memory turns rows from here on
-#pragma unroll
-    for (int j = 0; j < S::MQ; j++) {
-        if (wave_q + j * 16 >= a.q.rows) break;
-        f32x4 v[S::MP];
-#pragma unroll
-        for (int i = 0; i < S::MP; i++) v[i] = acc[i][j];
-        turn_rows<S>((uint32_t)(uintptr_t)(GM_LDS char *)tiles, v, [&](int row, int p, float (&out)[8]) {
-            const int q = wave_q + j * 16 + row;
-            p += wave_p;
-            if (q >= a.q.rows || p >= a.p.rows) return;
-            if (a.splits > 1) {
-                const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
-                store8(a.partial + ((int64_t)split * a.most + q) * a.p.rows + p, count == 8 && a.p.rows % 4 == 0, count, out);
-            } else {
-                finish(a, by, q, p, out);
-            }
-        });
-    }
+    store_tile<S>(a, a.head->coefficient * a.unscale, p0, q0, split, product.turn_place(), acc);
 }
 
 // The parts of a split sum, added up in order; eight outputs a lane.
@@ -476,12 +522,14 @@ struct LossPlan {
 // rows a large power of two apart would all lie on the same channel of the L2.
 constexpr int kSkew = 64;
 
+
 constexpr int kLeastChunk = 256;
 constexpr size_t kKeptBytes = (size_t)4 << 30;      // of exp(s - m) and dS together, unless one chunk needs more
 
 static int shape_for(int64_t p, int64_t q)
 {
     if (q <= kShapeQ[kFlat]) return kFlat;
+    if (q <= kShapeQ[kTall]) return kTall;
     // a wide tile needs a CU to itself: with fewer of them than CUs the smaller ones are spread better
     return ((p + 255) / 256) * ((q + 255) / 256) >= 256 ? kWide : kSquare;
 }
@@ -520,14 +568,13 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
         // long as a part is worth a tile's beginning and end
         const int steps = s.padded / kStepK * (s.planes == 3 ? 6 : 1);
         const auto parts = [&](int shape) {
-            const int want = (shape == kWide ? 256 : 512) / tiles(shape, dim, s.chunk), most = steps / 16;
+            const int want = (shape == kWide || shape == kTall ? 256 : 512) / tiles(shape, dim, s.chunk), most = steps / 16;
             return want < 1 || most < 1 ? 1 : want < most ? want : most;
         };
         s.dx_shape = shape_for(dim, s.chunk);
         if (s.dx_shape == kSquare && tiles(kWide, dim, s.chunk) * parts(kWide) >= 192) s.dx_shape = kWide;
         s.dx_splits = parts(s.dx_shape);
-        s.dw_shape = shape_for(dim, vocab);
-        if (s.dw_shape == kFlat) s.dw_shape = kSquare;
+        s.dw_shape = tiles(kWide, dim, vocab) >= 256 ? kWide : kSquare;
     }
     const size_t rows = up((size_t)n, kStepK), chunk_rows = up((size_t)s.chunk, kStepK);
     size_t at = 0;
@@ -587,6 +634,7 @@ static void launch_logits(int shape, const LogitsArgs &a, int rows, hipStream_t 
     const int grid = (tiles(shape, a.vocab, rows) + 7) / 8 * 8;
     if (shape == kWide) logits_kernel<T, WideShape><<<grid, WideShape::THREADS, 0, stream>>>(a);
     else if (shape == kSquare) logits_kernel<T, SquareShape><<<grid, SquareShape::THREADS, 0, stream>>>(a);
+    else if (shape == kTall) logits_kernel<T, TallShape><<<grid, TallShape::THREADS, 0, stream>>>(a);
     else logits_kernel<T, FlatShape><<<grid, FlatShape::THREADS, 0, stream>>>(a);
 }
 
@@ -596,7 +644,10 @@ static void launch_product(int shape, const ProductArgs &a, int p, int q, hipStr
     const unsigned grid = ((unsigned)tiles(shape, p, q) * a.splits + 7) / 8 * 8;
     if (shape == kWide) product_kernel<T, WideShape, DW><<<grid, WideShape::THREADS, 0, stream>>>(a);
     else if (shape == kSquare) product_kernel<T, SquareShape, DW><<<grid, SquareShape::THREADS, 0, stream>>>(a);
-    else if constexpr (!DW) product_kernel<T, FlatShape, DW><<<grid, FlatShape::THREADS, 0, stream>>>(a);
+    else if constexpr (!DW) {
+        if (shape == kTall) product_kernel<T, TallShape, DW><<<grid, TallShape::THREADS, 0, stream>>>(a);
+        else product_kernel<T, FlatShape, DW><<<grid, FlatShape::THREADS, 0, stream>>>(a);
+    }
 }
 
 // I: what the caller's tensors hold; T: what the matrix cores take.

@@ -170,165 +170,196 @@ struct Shape {
     static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STAGES = STAGES_;
     static constexpr int WAVES = WP * WQ, THREADS = WAVES * 64;
     static constexpr int MP = BP / WP / 16, MQ = BQ / WQ / 16;        // matrix instructions a wavefront, either way
-    static constexpr int LDS = (BP + BQ) * kStepK * 2 * STAGES;
+    static constexpr int LDS = (BP + BQ) * kStepK * 2 * STAGES;       // bytes of all stages
+    static constexpr int TURN = WQ * BP * 16 * 4;                     // bytes that turn_rows takes
+    static_assert(TURN <= LDS, "turning rows fits the stages' memory");
 };
 
-// The sum over steps [first, last) of the pairs' k; acc[i][j]: rows 16 i of P, 16 j of Q of this wavefront.
+// The sum over steps [first, last) of the pairs' k for one tile; acc[i][j]: rows 16 i of P, 16 j of Q of this wavefront.
 // steps: steps of one pair; limit_p / limit_q: the k that exist where an operand lies across.
 //
 // A step's matrix instructions come in two halves of 32 k, row by row of P's fragments.  A fragment of P is replaced by
 // the next half's as soon as its row is through, so reads from LDS run half a step ahead all the time.  Shortly after the
 // first half every wavefront has read all of its stage: one barrier there frees the stage for the loads of the step
 // STAGES later, and makes the next step's data, which have arrived by then, visible.
+//
 template <typename T, typename S, bool PACROSS, bool QACROSS>
-__device__ inline void multiply_tiles(const Operand &p, const Operand &q, const PlanePairs &pairs, int p0, int q0, int steps, int limit_p,
-                                      int limit_q, int first, int last, uint32_t lds, f32x4 (&acc)[S::MP][S::MQ])
-{
+struct Multiplier {
     typedef Tile<S::BP, PACROSS, S::WAVES> TP;
     typedef Tile<S::BQ, QACROSS, S::WAVES> TQ;
-    constexpr int kLoads = TP::kLoads + TQ::kLoads;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
-    const uint32_t lds_q = lds + S::STAGES * TP::kBytes;      // P's stages, then Q's
-    uint32_t off_p[TP::kLoads], off_q[TQ::kLoads];
-    TP::offsets(p, p0, wave, lane, off_p);
-    TQ::offsets(q, q0, wave, lane, off_q);
-    auto at_p = TP::template places<S::MP>(lds, wp, lane);
-    auto at_q = TQ::template places<S::MQ>(lds_q, wq, lane);
-#pragma unroll
-    for (int i = 0; i < S::MP; i++)
-#pragma unroll
-        for (int j = 0; j < S::MQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    static constexpr int kLoads = TP::kLoads + TQ::kLoads;
+    static constexpr int kMeet = S::MP >= 4 ? 1 : 0;      // the row of the second half that the barrier follows
+    // Q's fragments are all needed by the next half's first row: they are read behind the first rows
+    static constexpr int kEarly = S::MP >= 2 * S::MQ ? 1 : S::MP >= S::MQ ? 2 : S::MQ;
 
-    // the next step to load: its pair, its k, its addresses
-    int load_step = first, load_pair = first / steps, load_k = (first - load_pair * steps) * kStepK;
-    const int edge = (steps - 1) * kStepK;      // the k of a pair's last step
-    const int64_t ahead_p = PACROSS ? (int64_t)p.stride * (2 * kStepK) : 2 * kStepK, ahead_q = QACROSS ? (int64_t)q.stride * (2 * kStepK) : 2 * kStepK;
+    const Operand p, q;
+    const PlanePairs pairs;
+    const int steps, limit_p, limit_q, first, last, edge;      // edge: the k of a pair's last step; steps may run past the last pair's
+                                                               // end and go on at the first one's beginning
+    const uint32_t lds, lds_q;                                 // P's stages, then Q's
+    const int lane, wave;
+    int p0, q0;
+    uint32_t off_p[TP::kLoads], off_q[TQ::kLoads];
+    int load_step, load_pair, load_k;                          // the next step to load
     const char *from_p, *from_q;
-    const auto seek = [&]() {
+
+    __device__ inline Multiplier(const Operand &p_, const Operand &q_, const PlanePairs &pairs_, int steps_, int limit_p_, int limit_q_, int first_,
+                                 int last_, uint32_t lds_)
+        : p(p_), q(q_), pairs(pairs_), steps(steps_), limit_p(limit_p_), limit_q(limit_q_), first(first_), last(last_), edge((steps_ - 1) * kStepK),
+          lds(lds_), lds_q(lds_ + S::STAGES * TP::kBytes), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6))
+    {
+    }
+
+    __device__ inline void seek()
+    {
         const uint32_t code = pairs.codes >> (4 * load_pair);
         const short *bp = p.base + (int64_t)(code & 3) * p.plane, *bq = q.base + (int64_t)(code >> 2 & 3) * q.plane;
         from_p = reinterpret_cast<const char *>(PACROSS ? bp + (int64_t)load_k * p.stride + p0 : bp + (int64_t)p0 * p.stride + load_k);
         from_q = reinterpret_cast<const char *>(QACROSS ? bq + (int64_t)load_k * q.stride + q0 : bq + (int64_t)q0 * q.stride + load_k);
-    };
-    const auto at_edge = [&]() {
+    }
+    __device__ inline void at_edge()
+    {
         if (PACROSS && limit_p < edge + kStepK) TP::clamp(limit_p - edge, (uint32_t)p.stride * 2u, wave, lane, off_p);
         if (QACROSS && limit_q < edge + kStepK) TQ::clamp(limit_q - edge, (uint32_t)q.stride * 2u, wave, lane, off_q);
-    };
-    seek();
-    if (load_k == edge) at_edge();
-    const auto load_one = [&](int stage, int i) {      // i: which of this wavefront's loads
+    }
+    __device__ inline void load_one(int stage, int i)      // i: which of this wavefront's loads
+    {
         if (i < TP::kLoads) TP::load(from_p, off_p[i < TP::kLoads ? i : 0], lds + stage * TP::kBytes, wave, i);
         else TQ::load(from_q, off_q[i >= TP::kLoads ? i - TP::kLoads : 0], lds_q + stage * TQ::kBytes, wave, i - TP::kLoads);
-    };
-    const auto loaded = [&]() {
+    }
+    __device__ inline void loaded()
+    {
         load_step++;
         load_k += kStepK;
-        from_p += ahead_p;
-        from_q += ahead_q;
+        from_p += PACROSS ? (int64_t)p.stride * (2 * kStepK) : 2 * kStepK;
+        from_q += QACROSS ? (int64_t)q.stride * (2 * kStepK) : 2 * kStepK;
         if (load_k >= edge) {
             if (load_k > edge) {      // the next pair from its beginning
                 load_k = 0;
-                if (++load_pair < pairs.count) {
-                    seek();
-                    if (PACROSS && limit_p < edge + kStepK) TP::offsets(p, p0, wave, lane, off_p);
-                    if (QACROSS && limit_q < edge + kStepK) TQ::offsets(q, q0, wave, lane, off_q);
-                }
+                load_pair = load_pair + 1 < pairs.count ? load_pair + 1 : 0;
+                seek();
+                if (PACROSS && limit_p < edge + kStepK) TP::offsets(p, p0, wave, lane, off_p);
+                if (QACROSS && limit_q < edge + kStepK) TQ::offsets(q, q0, wave, lane, off_q);
             }
             if (load_k == edge) at_edge();
         }
-    };
-#pragma unroll
-    for (int s = 0; s < S::STAGES; s++)
-        if (load_step < last) {
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) load_one(s, i);
-            loaded();
-        }
-    if (first + S::STAGES <= last) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S::STAGES - 1) * kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+    }
 
-    s16x8 fp[S::MP], fq[2][S::MQ];
-    constexpr int kMeet = S::MP >= 4 ? 1 : 0;      // the row of the second half that the barrier follows
-    // The order is pinned (sched_barrier): left to itself the compiler gathers the reads in front of their first use, and the
-    // matrix cores wait for them.
-    const auto row = [&](int half, int i) {
-        __builtin_amdgcn_sched_barrier(0);
+    // Every wavefront of the workgroup must be done with the tiles in LDS.
+    __device__ inline void start(int p0_, int q0_)
+    {
+        p0 = p0_, q0 = q0_;
+        TP::offsets(p, p0, wave, lane, off_p);
+        TQ::offsets(q, q0, wave, lane, off_q);
+        load_step = first, load_pair = first / steps, load_k = (first - load_pair * steps) * kStepK;
+        seek();
+        if (load_k == edge) at_edge();
 #pragma unroll
-        for (int j = 0; j < S::MQ; j++) acc[i][j] = multiply_add<T>(fp[i], fq[half][j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    // Q's fragments are all needed by the next half's first row: they are read behind the first rows
-    constexpr int kEarly = S::MP >= 2 * S::MQ ? 1 : S::MP >= S::MQ ? 2 : S::MQ;
-    int stage = 0;
-    // `more`: a step is left to load, and all stages are under way
-    const auto whole_step = [&](auto more) {
+        for (int s = 0; s < S::STAGES; s++)
+            if (load_step < last) {
 #pragma unroll
-        for (int i = 0; i < S::MP; i++) {      // the first half; the second one's fragments are read
-            row(0, i);
-#pragma unroll
-            for (int j = i * kEarly; j < (i + 1) * kEarly && j < S::MQ; j++) fq[1][j] = TQ::fragment(at_q, j, 1);
-            fp[i] = TP::fragment(at_p, i, 1);
-        }
-        const bool wraps = stage == S::STAGES - 1;
-        TP::move(at_p, wraps ? -(S::STAGES - 1) * TP::kBytes : TP::kBytes);
-        TQ::move(at_q, wraps ? -(S::STAGES - 1) * TQ::kBytes : TQ::kBytes);
-#pragma unroll
-        for (int i = 0; i < S::MP; i++) {      // the second half; the next step's first half is read
-            row(1, i);
-            if (i < kMeet) continue;
-            if (i == kMeet) {
-                if constexpr (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::STAGES - 2) * kLoads) : "memory");
-                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
+                for (int i = 0; i < kLoads; i++) load_one(s, i);
+                loaded();
             }
-            constexpr int kRows = S::MP - kMeet;
-            const int at = i - kMeet;
+    }
+
+    // Where turn_rows may work for this wavefront, after run().
+    __device__ inline uint32_t turn_place() const { return lds + wave * (S::BP / S::WP * 16 * 4); }
+
+    __device__ inline void run(f32x4 (&acc)[S::MP][S::MQ])
+    {
+        const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
+        auto at_p = TP::template places<S::MP>(lds, wp, lane);
+        auto at_q = TQ::template places<S::MQ>(lds_q, wq, lane);
 #pragma unroll
-            for (int j = at * kEarly; j < (at + 1) * kEarly && j < S::MQ; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
+        for (int i = 0; i < S::MP; i++)
 #pragma unroll
-            for (int r = i == kMeet ? 0 : i; r <= i; r++) fp[r] = TP::fragment(at_p, r, 0);
-            if constexpr (more) {
+            for (int j = 0; j < S::MQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (first + S::STAGES <= last) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S::STAGES - 1) * kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+
+        s16x8 fp[S::MP], fq[2][S::MQ];
+        // The order is pinned (sched_barrier): left to itself the compiler gathers the reads in front of their first use, and the
+        // matrix cores wait for them.
+        const auto row = [&](int half, int i) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int l = at * kLoads / kRows; l < (at + 1) * kLoads / kRows; l++) load_one(stage, l);
+            for (int j = 0; j < S::MQ; j++) acc[i][j] = multiply_add<T>(fp[i], fq[half][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        int stage = 0;
+        // `more`: a step is left to load, and all stages are under way
+        const auto whole_step = [&](auto more) {
+#pragma unroll
+            for (int i = 0; i < S::MP; i++) {      // the first half; the second one's fragments are read
+                row(0, i);
+#pragma unroll
+                for (int j = i * kEarly; j < (i + 1) * kEarly && j < S::MQ; j++) fq[1][j] = TQ::fragment(at_q, j, 1);
+                fp[i] = TP::fragment(at_p, i, 1);
             }
-        }
-        if constexpr (more) loaded();
-        stage = wraps ? 0 : stage + 1;
-    };
+            const bool wraps = stage == S::STAGES - 1;
+            TP::move(at_p, wraps ? -(S::STAGES - 1) * TP::kBytes : TP::kBytes);
+            TQ::move(at_q, wraps ? -(S::STAGES - 1) * TQ::kBytes : TQ::kBytes);
 #pragma unroll
-    for (int j = 0; j < S::MQ; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
+            for (int i = 0; i < S::MP; i++) {      // the second half; the next step's first half is read
+                row(1, i);
+                if (i < kMeet) continue;
+                if (i == kMeet) {
+                    if constexpr (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::STAGES - 2) * kLoads) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                }
+                constexpr int kRows = S::MP - kMeet;
+                const int at = i - kMeet;
 #pragma unroll
-    for (int i = 0; i < S::MP; i++) fp[i] = TP::fragment(at_p, i, 0);
-    int step = first;
-    for (; step + S::STAGES < last; step++) whole_step(std::true_type());
-    for (; step < last; step++) whole_step(std::false_type());
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-}
+                for (int j = at * kEarly; j < (at + 1) * kEarly && j < S::MQ; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
+#pragma unroll
+                for (int r = i == kMeet ? 0 : i; r <= i; r++) fp[r] = TP::fragment(at_p, r, 0);
+                if constexpr (more) {
+#pragma unroll
+                    for (int l = at * kLoads / kRows; l < (at + 1) * kLoads / kRows; l++) load_one(stage, l);
+                }
+            }
+            if constexpr (more) loaded();
+            stage = wraps ? 0 : stage + 1;
+        };
+#pragma unroll
+        for (int j = 0; j < S::MQ; j++) fq[0][j] = TQ::fragment(at_q, j, 0);
+#pragma unroll
+        for (int i = 0; i < S::MP; i++) fp[i] = TP::fragment(at_p, i, 0);
+        int step = first;
+        for (; step + S::STAGES < last; step++) whole_step(std::true_type());
+        for (; step < last; step++) whole_step(std::false_type());
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();      // everyone is done with the tiles
+    }
+};
 
 // Sixteen rows of Q's outputs go through the wavefront's own share of LDS on their way out: a lane holds four p of one q,
 // and what it would store is 8 bytes of each of sixteen rows; turned, a wavefront stores whole rows of its p, 16 bytes a
-// lane.  `use(row, p, v)` gets eight consecutive p (from the wavefront's first) of row 0 .. 15.  Every wavefront of the
-// workgroup must be done with the tiles in LDS.
+// lane.  `use(row, p, v)` gets eight consecutive p (from the wavefront's first) of row 0 .. 15.  Pieces of 16 bytes of
+// row r lie at their number XOR r, so that neither side meets on a bank.  mine: memory of this wavefront's own.
+template <typename S>
+constexpr int kTurnRows = 64 / (S::BP / S::WP / 8);
+
 template <typename S, typename F>
-__device__ inline void turn_rows(uint32_t lds, const f32x4 (&v)[S::MP], F &&use)
+__device__ inline void turn_rows(uint32_t mine, const f32x4 (&v)[S::MP], F &&use)
 {
-    constexpr int kSpan = S::BP / S::WP, kPitch = kSpan * 4 + 16, kLanes = kSpan / 8, kRows = 64 / kLanes;
-    static_assert(S::WAVES * 16 * kPitch <= S::LDS, "room for every wavefront");
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t mine = lds + wave * (16 * kPitch);
+    constexpr int kSpan = S::BP / S::WP, kPitch = kSpan * 4, kLanes = kSpan / 8, kRows = kTurnRows<S>, kMask = kSpan / 4 - 1 < 15 ? kSpan / 4 - 1 : 15;
+    const int lane = threadIdx.x & 63, to = lane & 15;
 #pragma unroll
-    for (int i = 0; i < S::MP; i++) *reinterpret_cast<GM_LDS f32x4 *>(mine + (lane & 15) * kPitch + (i * 16 + (lane >> 4) * 4) * 4) = v[i];
+    for (int i = 0; i < S::MP; i++)
+        *reinterpret_cast<GM_LDS f32x4 *>(mine + to * kPitch + (((i * 4 + (lane >> 4)) ^ (to & kMask)) << 4)) = v[i];
 #pragma unroll
     for (int pass = 0; pass < 16 / kRows; pass++) {
-        const int row = pass * kRows + lane / kLanes, p = lane % kLanes * 8;
-        const GM_LDS f32x4 *at = reinterpret_cast<const GM_LDS f32x4 *>(mine + row * kPitch + p * 4);
-        const f32x4 a = at[0], b = at[1];
+        const int row = pass * kRows + lane / kLanes, piece = lane % kLanes * 2;
+        const f32x4 a = *reinterpret_cast<const GM_LDS f32x4 *>(mine + row * kPitch + ((piece ^ (row & kMask)) << 4));
+        const f32x4 b = *reinterpret_cast<const GM_LDS f32x4 *>(mine + row * kPitch + (((piece + 1) ^ (row & kMask)) << 4));
         float out[8];
 #pragma unroll
         for (int e = 0; e < 4; e++) out[e] = a[e], out[4 + e] = b[e];
-        use(row, p, out);
+        use(row, piece * 4, out);
     }
 }
 
