@@ -93,22 +93,23 @@ scan_targets_kernel(const int *targets, int n, int vocab, int ignore, int mean, 
     }
 }
 
-// x as the planes of an operand: h, then what of x is left after h, and so on; each rounded to nearest.
+// Eight elements as the planes of an operand: rounded to nearest, then what is left of them after that, and so on.
 template <typename T>
-__device__ inline void split_store(float x, T *to, int64_t plane, int planes)
+__device__ inline void split_store(float (&v)[8], T *to, int64_t plane, int planes)
 {
     for (int k = 0; k < planes; k++) {
-        const T part = from_float<T>(x);
-        to[k * plane] = part;
-        x = x - (float)part;
+        store8(to + k * plane, true, 8, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = v[e] - (float)from_float<T>(v[e]);
     }
 }
 
-// Rows of a matrix as operand rows: `width` elements (a multiple of 64) of each, zeros behind the matrix's own `dim`.
-template <typename I, typename T>
-__device__ inline void pack_row(const I *from, T *to, int dim, int width, int64_t plane, int planes)
+// Eight elements of a matrix's row of `dim`, zeros behind it.
+template <typename I>
+__device__ inline void load_padded(const I *row, int c, int dim, bool aligned, float (&v)[8])
 {
-    for (int c = threadIdx.x; c < width; c += blockDim.x) split_store<T>(from && c < dim ? (float)from[c] : 0.0f, to + c, plane, planes);
+    const int count = dim - c < 8 ? (dim - c < 0 ? 0 : dim - c) : 8;
+    load8(row + c, aligned && count == 8, count, v);
 }
 
 constexpr int kPackBlock = 256;
@@ -117,18 +118,24 @@ constexpr int kPackBlock = 256;
 // token, up to a whole step of k, become zeros.
 template <typename I, typename T>
 __global__ void __launch_bounds__(kPackBlock)
-pack_tokens_kernel(const I *x, int64_t x_stride, int n, int dim, int width, const LossHead *head, const int *place_of, T *packed,
+pack_tokens_kernel(const I *x, int64_t x_stride, bool aligned, int n, int dim, int width, const LossHead *head, const int *place_of, T *packed,
                    int64_t packed_stride, int64_t plane, int planes, float *losses, I *dx, int64_t dx_stride)
 {
     const int i = blockIdx.x;
     if (i >= n) {
         const int r = head->count + (i - n), end = (head->count + kStepK - 1) / kStepK * kStepK;
-        if (r < end) pack_row<I, T>(nullptr, packed + r * packed_stride, 0, width, plane, planes);
+        float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < end)
+            for (int c = threadIdx.x * 8; c < width; c += kPackBlock * 8) split_store<T>(zero, packed + r * packed_stride + c, plane, planes);
         return;
     }
     const int place = place_of[i];
     if (place >= 0) {
-        pack_row<I, T>(x + (int64_t)i * x_stride, packed + place * packed_stride, dim, width, plane, planes);
+        for (int c = threadIdx.x * 8; c < width; c += kPackBlock * 8) {
+            float v[8];
+            load_padded(x + (int64_t)i * x_stride, c, dim, aligned, v);
+            split_store<T>(v, packed + place * packed_stride + c, plane, planes);
+        }
         return;
     }
     if (threadIdx.x == 0) losses[i] = 0.0f;
@@ -136,11 +143,19 @@ pack_tokens_kernel(const I *x, int64_t x_stride, int n, int dim, int width, cons
         for (int c = threadIdx.x; c < dim; c += kPackBlock) dx[(int64_t)i * dx_stride + c] = (I)0.0f;
 }
 
+// The weights as operand rows of `width` elements (a multiple of 64), eight a lane.
 template <typename I, typename T>
 __global__ void __launch_bounds__(kPackBlock)
-pack_weights_kernel(const I *w, int64_t w_stride, int dim, int width, T *packed, int64_t plane, int planes)
+pack_weights_kernel(const I *w, int64_t w_stride, bool aligned, int rows, int dim, int width, T *packed, int64_t plane, int planes)
 {
-    pack_row<I, T>(w + (int64_t)blockIdx.x * w_stride, packed + (int64_t)blockIdx.x * width, dim, width, plane, planes);
+    const int per_row = width / 8;
+    const int64_t first = (int64_t)blockIdx.x * kPackBlock;
+    const int first_row = (int)(first / per_row), at = (int)(first - (int64_t)first_row * per_row) + (int)threadIdx.x;
+    const int row = first_row + at / per_row, c = at % per_row * 8;
+    if (row >= rows) return;
+    float v[8];
+    load_padded(w + row * w_stride, c, dim, aligned, v);
+    split_store<T>(v, packed + (int64_t)row * width + c, plane, planes);
 }
 
 // --------------------------------------------------------------------------------------------------- logits ----
@@ -341,7 +356,8 @@ struct ProductArgs {
     int steps;                       // steps of 64 k of one pair; 0: as many as the chunk has tokens (dW)
     int limit_p;                     // across: the k that exist
     int splits;                      // parts of the sum; more than one: `partial` takes them
-    float *partial;                  // [split][most][p rows]
+    float *partial;                  // [split][partial_rows][p rows]
+    int partial_rows;                // at least as many as q has
     const LossHead *head;
     const int *row_of;               // dX: where a packed row belongs
     float unscale;                   // undoes kSlopeScale
@@ -417,7 +433,7 @@ __device__ inline void store_tile(const ProductArgs &a, float by, int p0, int q0
     const int wave_p = p0 + wave / S::WQ * (S::BP / S::WP), wave_q = q0 + wave % S::WQ * (S::BQ / S::WQ);
     if (wave_p + S::BP / S::WP <= a.p.rows && wave_q + S::BQ / S::WQ <= a.q.rows) {
         if (a.splits > 1 && a.p.rows % 4 == 0) {
-            store_whole<S>(a.partial + ((int64_t)split * a.most + wave_q) * a.p.rows + wave_p, a.p.rows, 1.0f, turn, acc);
+            store_whole<S>(a.partial + ((int64_t)split * a.partial_rows + wave_q) * a.p.rows + wave_p, a.p.rows, 1.0f, turn, acc);
             return;
         }
         if (a.splits == 1 && a.out_aligned && !a.accumulate && !a.add && !a.row_of) {
@@ -440,7 +456,7 @@ __device__ inline void store_tile(const ProductArgs &a, float by, int p0, int q0
             if (q >= a.q.rows || p >= a.p.rows) return;
             if (a.splits > 1) {
                 const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
-                store8(a.partial + ((int64_t)split * a.most + q) * a.p.rows + p, count == 8 && a.p.rows % 4 == 0, count, out);
+                store8(a.partial + ((int64_t)split * a.partial_rows + q) * a.p.rows + p, count == 8 && a.p.rows % 4 == 0, count, out);
             } else {
                 finish(a, by, q, p, out);
             }
@@ -483,7 +499,8 @@ product_kernel(ProductArgs a)
 __global__ void __launch_bounds__(256)
 join_splits_kernel(ProductArgs a)
 {
-    const int rows = chunk_rows(a.head, a.first, a.most);
+    const int tokens = chunk_rows(a.head, a.first, a.most), rows = a.row_of ? tokens : a.q.rows;
+    if (tokens == 0 && a.skip_empty) return;
     const int per_row = (a.p.rows + 7) / 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int q = (int)(i / per_row), p = (int)(i - (int64_t)q * per_row) * 8;
@@ -495,7 +512,7 @@ join_splits_kernel(ProductArgs a)
     for (int s = 0; s < a.splits; s += kAhead) {
         float v[kAhead][8];
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) load8(a.partial + ((int64_t)(s + k < a.splits ? s + k : s) * a.most + q) * a.p.rows + p, whole, count, v[k]);
+        for (int k = 0; k < kAhead; k++) load8(a.partial + ((int64_t)(s + k < a.splits ? s + k : s) * a.partial_rows + q) * a.p.rows + p, whole, count, v[k]);
 #pragma unroll
         for (int k = 0; k < kAhead; k++)
             if (s + k < a.splits) {
@@ -514,7 +531,7 @@ struct LossPlan {
     int operand_type;                      // kFloat16 or kBFloat16
     int planes, slope_planes, keep;        // planes of x (and W); of dS
     bool gradients, pack_weights, sum_weights;      // sum_weights: dW of several chunks in 16 bits needs fp32 sums
-    int logits_shape, groups, dx_shape, dx_splits, dw_shape;
+    int logits_shape, groups, dx_shape, dx_splits, dw_shape, dw_splits;
     size_t head, row_of, place_of, row_target, target_logit, x, w, stats, kept, slopes, partial, sums, bytes;
 };
 
@@ -526,17 +543,24 @@ constexpr int kSkew = 64;
 constexpr int kLeastChunk = 256;
 constexpr size_t kKeptBytes = (size_t)4 << 30;      // of exp(s - m) and dS together, unless one chunk needs more
 
-static int shape_for(int64_t p, int64_t q)
-{
-    if (q <= kShapeQ[kFlat]) return kFlat;
-    if (q <= kShapeQ[kTall]) return kTall;
-    // a wide tile needs a CU to itself: with fewer of them than CUs the smaller ones are spread better
-    return ((p + 255) / 256) * ((q + 255) / 256) >= 256 ? kWide : kSquare;
-}
-
 static int tiles(int shape, int64_t p, int64_t q)
 {
     return (int)(((p + kShapeP[shape] - 1) / kShapeP[shape]) * ((q + kShapeQ[shape] - 1) / kShapeQ[shape]));
+}
+
+// Whether wide tiles finish first.  They come in rounds of 256, one a CU; square ones in rounds of 512, two a CU, that take 0.83
+// of a wide round (a quarter of the outputs each, at 0.6 of the rate: their fragments are read from LDS twice as often).
+// 300 x 30000 x 1024 fp32, logits: 236 wide tiles 184 us, 705 square ones 210 us; dW of 10007 x 1000: 160 wide tiles instead of
+// 632 square ones take 20 us off 100.
+static int wide_or_square(int64_t p, int64_t q)
+{
+    const int wide = (tiles(kWide, p, q) + 255) / 256, square = (tiles(kSquare, p, q) + 511) / 512;
+    return wide * 100 <= square * 83 ? kWide : kSquare;
+}
+
+static int shape_for(int64_t p, int64_t q)
+{
+    return q <= kShapeQ[kFlat] ? kFlat : q <= kShapeQ[kTall] ? kTall : wide_or_square(p, q);
 }
 
 static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_type, int gradient_type, bool gradients, int chunk)
@@ -565,16 +589,19 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.groups = (vocab + kShapeP[s.logits_shape] - 1) / kShapeP[s.logits_shape] * (kShapeP[s.logits_shape] / kShapeSpan[s.logits_shape]);
     if (gradients) {
         // few outputs, a long sum: parts of it until every CU has work (two workgroups of the smaller shapes fit a CU), as
-        // long as a part is worth a tile's beginning and end
-        const int steps = s.padded / kStepK * (s.planes == 3 ? 6 : 1);
-        const auto parts = [&](int shape) {
-            const int want = (shape == kWide || shape == kTall ? 256 : 512) / tiles(shape, dim, s.chunk), most = steps / 16;
-            return want < 1 || most < 1 ? 1 : want < most ? want : most;
+        // long as a part is worth a tile's beginning and end; wide tiles where their parts fill the chip
+        const auto split = [](int &shape, int &splits, int64_t p, int64_t q, int steps) {
+            const auto parts = [&](int of) {
+                const int want = (of == kWide || of == kTall ? 256 : 512) / tiles(of, p, q), most = steps / 16;
+                return want < 1 || most < 1 ? 1 : want < most ? want : most;
+            };
+            if (shape == kSquare && tiles(kWide, p, q) * parts(kWide) >= 192) shape = kWide;
+            splits = parts(shape);
         };
         s.dx_shape = shape_for(dim, s.chunk);
-        if (s.dx_shape == kSquare && tiles(kWide, dim, s.chunk) * parts(kWide) >= 192) s.dx_shape = kWide;
-        s.dx_splits = parts(s.dx_shape);
-        s.dw_shape = tiles(kWide, dim, vocab) >= 256 ? kWide : kSquare;
+        split(s.dx_shape, s.dx_splits, dim, s.chunk, s.padded / kStepK * (s.planes == 3 ? 6 : 1));
+        s.dw_shape = wide_or_square(dim, vocab);
+        split(s.dw_shape, s.dw_splits, dim, vocab, (s.chunk + kStepK - 1) / kStepK * (s.planes == 3 ? 6 : s.slope_planes));
     }
     const size_t rows = up((size_t)n, kStepK), chunk_rows = up((size_t)s.chunk, kStepK);
     size_t at = 0;
@@ -590,7 +617,10 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.stats = take(sizeof(float2) * (size_t)s.chunk * s.groups);
     s.kept = take(s.keep == kKeepNothing ? 0 : chunk_rows * s.slope_stride * (s.keep == kKeepHalf ? 2 : 4));
     s.slopes = s.keep == kKeepFloat ? take(chunk_rows * s.slope_stride * 2 * s.slope_planes) : s.kept;
-    s.partial = take(gradients && s.dx_splits > 1 ? (size_t)s.dx_splits * s.chunk * dim * 4 : 0);
+    // (dX is joined before dW's parts are written)
+    const size_t dx_parts = gradients && s.dx_splits > 1 ? (size_t)s.dx_splits * s.chunk * dim * 4 : 0;
+    const size_t dw_parts = gradients && s.dw_splits > 1 ? (size_t)s.dw_splits * vocab * dim * 4 : 0;
+    s.partial = take(dx_parts > dw_parts ? dx_parts : dw_parts);
     s.sums = take(s.sum_weights ? (size_t)vocab * dim * 4 : 0);
     s.bytes = at;
     return s;
@@ -648,6 +678,7 @@ static void launch_product(int shape, const ProductArgs &a, int p, int q, hipStr
         if (shape == kTall) product_kernel<T, TallShape, DW><<<grid, TallShape::THREADS, 0, stream>>>(a);
         else product_kernel<T, FlatShape, DW><<<grid, FlatShape::THREADS, 0, stream>>>(a);
     }
+    if (a.splits > 1) join_splits_kernel<<<(unsigned)(((int64_t)q * ((p + 7) / 8) + 255) / 256), 256, 0, stream>>>(a);
 }
 
 // I: what the caller's tensors hold; T: what the matrix cores take.
@@ -666,13 +697,16 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
 
     scan_targets_kernel<<<1, kScanBlock, 0, stream>>>(reinterpret_cast<const int *>(c.targets), s.n, s.vocab, c.ignore, c.mean,
                                                       c.gradient_scale, c.amp, head, row_of, place_of, row_target);
-    pack_tokens_kernel<I, T><<<s.n + kStepK, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.hidden), c.hidden_stride, s.n, s.dim,
+    pack_tokens_kernel<I, T><<<s.n + kStepK, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.hidden), c.hidden_stride,
+                                                                      c.hidden % 16 == 0 && c.hidden_stride * sizeof(I) % 16 == 0, s.n, s.dim,
                                                                       s.width, head, place_of, x, s.x_stride, x_plane, s.planes, losses,
                                                                       reinterpret_cast<I *>(c.dx), c.dx_stride);
     Operand w{reinterpret_cast<const short *>(c.weight), c.weight_stride, 0, s.vocab};
     if (s.pack_weights) {
-        pack_weights_kernel<I, T><<<s.vocab, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight), c.weight_stride, s.dim, s.width,
-                                                                      reinterpret_cast<T *>(space + s.w), w_plane, s.planes);
+        const unsigned grid = (unsigned)(((int64_t)s.vocab * (s.width / 8) + kPackBlock - 1) / kPackBlock);
+        pack_weights_kernel<I, T><<<grid, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight), c.weight_stride,
+                                                                   c.weight % 16 == 0 && c.weight_stride * sizeof(I) % 16 == 0, s.vocab, s.dim,
+                                                                   s.width, reinterpret_cast<T *>(space + s.w), w_plane, s.planes);
         w = Operand{reinterpret_cast<const short *>(space + s.w), s.width, w_plane, s.vocab};
     }
     const PlanePairs pairs = s.planes == 3 ? kSixPairs : kOnePair;
@@ -696,19 +730,18 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
             ProductArgs a{};
             a.p = w, a.p.rows = s.dim, a.q = slopes, a.pairs = pairs;
             a.first = first, a.most = tokens, a.steps = s.padded / kStepK, a.limit_p = s.vocab;
-            a.splits = s.dx_splits, a.partial = reinterpret_cast<float *>(space + s.partial);
+            a.splits = s.dx_splits, a.partial = reinterpret_cast<float *>(space + s.partial), a.partial_rows = tokens;
             a.head = head, a.row_of = row_of, a.unscale = 1.0f / kSlopeScale<T>;
             a.out = reinterpret_cast<void *>(c.dx), a.out_stride = c.dx_stride, a.out_type = c.data_type;
             a.out_aligned = c.dx % 16 == 0 && c.dx_stride * sizeof(I) % 16 == 0;
             launch_product<T, false>(s.dx_shape, a, s.dim, tokens, stream);
-            if (s.dx_splits > 1)
-                join_splits_kernel<<<(unsigned)(((int64_t)tokens * ((s.dim + 7) / 8) + 255) / 256), 256, 0, stream>>>(a);
         }
         if (c.dw) {
             ProductArgs a{};
             a.p = xs, a.p.rows = s.dim, a.q = slopes, a.q.rows = s.vocab;
             a.pairs = s.planes == 3 ? kSixPairs : s.slope_planes == 3 ? kThreeSlopes : s.slope_planes == 2 ? kTwoSlopes : kOnePair;
-            a.first = first, a.most = tokens, a.splits = 1, a.head = head, a.unscale = 1.0f / kSlopeScale<T>;
+            a.first = first, a.most = tokens, a.head = head, a.unscale = 1.0f / kSlopeScale<T>;
+            a.splits = s.dw_splits, a.partial = reinterpret_cast<float *>(space + s.partial), a.partial_rows = s.vocab;
             const bool last = k + 1 == s.chunks;
             float *sums = reinterpret_cast<float *>(space + s.sums);
             if (s.sum_weights && !last) {

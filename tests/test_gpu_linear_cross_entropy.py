@@ -109,6 +109,18 @@ def test_many_tokens(t, o):
         check(run(b, t, o, x, w, targets, scale=1024.0), t, o, x, w, targets, scale=1024.0)
 
 
+@pytest.mark.parametrize("t, o", PAIRS)
+@pytest.mark.parametrize("add", [False, True])
+def test_split_sums_of_the_weight_gradient(t, o, add):
+    """Few words and many tokens: the sum over the tokens is cut into parts, more of them than a batch of which few count fills."""
+    v, d = 130, 70
+    for n, ignored in ((2500, 0.1), (2500, 0.99)):
+        x, w, targets = data(t, n, v, d, ignored=ignored)
+        before = to_bits(np.random.default_rng(2).normal(size=(v, d)), o) if add else None
+        with Buffers() as b:
+            check(run(b, t, o, x, w, targets, scale=8.0, add=before), t, o, x, w, targets, scale=8.0, add=before)
+
+
 def test_wide_tiles_of_the_hidden_gradient():
     n, v, d = 4097, 300, 4100
     x, w, targets = data(BF16, n, v, d)
