@@ -372,6 +372,54 @@ def bench_placement(args, pkg, dev):
     print(json.dumps(result))
 
 
+def bench_lm_ends(args, pkg, dev):
+    """The operators at the two ends of a language model's training step, fp16, on random data: lookup and residual
+    dropout (HBM-bound), the table's gradient and the linear cross entropy with both gradients (matrix-core-bound)."""
+    lib, D = dev.lib, dev.handle
+    n, v, d, half = 4096, 131072, 4096, 2
+    rng = np.random.default_rng(9)
+    table, dtable, x, y, dx = (dev.alloc(2 * rows * d) for rows in (v, v, n, n, n))
+    lib.gm_fill_normal_f16(D, table, v * d, 0x61, 0.0, 0.02, 1.0)
+    lib.gm_fill_normal_f16(D, x, n * d, 0x62, 0.0, 1.0, 1.0)
+    tokens, targets = (dev.from_numpy(rng.integers(0, v, n).astype(np.int32)) for _ in range(2))
+    state, losses, loss = dev.from_numpy(np.array([1, 2, 3, 0], np.uint32)), dev.alloc(4 * n), dev.alloc(8)
+    sizes = [lib.gm_linear_cross_entropy_workspace(n, v, d, table, d, half, half, 1), lib.gm_embedding_gradient_workspace(n, v, d)]
+    space = [lib.gm_allocate_workspace(D, size) for size in sizes]
+
+    def checked(rc):
+        if rc != 0:
+            raise RuntimeError(f"rc={rc}: {lib.gm_last_error().decode()}")
+
+    cases = {
+        "execute_embedding_lookup, dropout": (lambda: checked(lib.execute_embedding_lookup(
+            D, 0, table, tokens, y, n, v, d, d, d, half, 64.0, 0.1, state, 0)), 4 * n * d, 0),
+        "execute_dropout, residual": (lambda: checked(lib.execute_dropout(D, 0, x, y, y, n * d, half, 0.1, state, 1)), 6 * n * d, 0),
+        "execute_linear_cross_entropy, both gradients": (lambda: checked(lib.execute_linear_cross_entropy(
+            D, 0, x, table, targets, losses, loss, dx, dtable, n, v, d, d, d, d, d, half, half, -100, 1, 65536.0, 0, 0, space[0], sizes[0])),
+            4 * (n + v) * d, 6 * n * v * d),
+        "execute_embedding_gradient": (lambda: checked(lib.execute_embedding_gradient(
+            D, 0, dx, tokens, dtable, n, v, d, d, d, half, half, 64.0, -1, 0, 0.1, state, 0, space[1], sizes[1])), 2 * (n + v) * d, 0),
+    }
+    records = {}
+    for name, (launch, nbytes, flops) in cases.items():
+        wall_ms, event_ms = time_steps(dev, launch, args.steps, args.warmup)
+        records[name] = {"bytes": nbytes, "flops": flops, "kernel_ms": event_ms, "ms_per_call": wall_ms,
+                         "achieved_gbs": nbytes / (event_ms * 1e-3) / 1e9, "achieved_tflops": flops / (event_ms * 1e-3) / 1e12}
+        print(f"{name}: {event_ms:.4f} ms", file=sys.stderr, flush=True)
+    head = records["execute_linear_cross_entropy, both gradients"]
+    result = {"metric": "TFLOP/s of the linear cross entropy with its gradients", "value": head["achieved_tflops"], "unit": "TFLOP/s",
+              "n_gpus": 1, "steps": args.steps, "warmup": args.warmup, "ms_per_step": head["ms_per_call"], "higher_is_better": True,
+              "scaling": "weak", "vs_baseline": None, "dtype": "f16", "data": "synthetic",
+              "config": {"workload": f"{n} tokens, {v} words, dimension {d}", "tokens": n, "vocab": v, "dim": d},
+              "roofline": {"bound": "matrix cores", "achieved": head["achieved_tflops"], "peak": 2500.0, "unit": "TFLOP/s",
+                           "frac": head["achieved_tflops"] / 2500.0},
+              "operators": records}
+    for h in space:
+        lib.deallocate_metal_buffer(h)
+    dev.close()
+    print(json.dumps(result))
+
+
 def bench_primitives(args, pkg, dev):
     """Buffer primitives of the boundary on one large buffer each: zero fill, fp32 <-> fp16 conversion,
     device-to-device copy (HBM-bound, timed with HIP events on the library's stream) and the host copies
@@ -598,7 +646,7 @@ def main():
     ap.add_argument("--gpus", type=int, default=1)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
-    ap.add_argument("--workload", default="", choices=[""] + sorted(WORKLOADS) + sorted(LBFGS_WORKLOADS) + ["primitives", "placement", "all"],
+    ap.add_argument("--workload", default="", choices=[""] + sorted(WORKLOADS) + sorted(LBFGS_WORKLOADS) + ["primitives", "placement", "lm-ends", "all"],
                     help="one workload in this process.  Default: the five benchmark configurations in turn, each in a "
                          "process of its own; the line printed is the headline configuration's (c5) with the others "
                          "under 'configs'.  'all': the same plus the L-BFGS workloads and the buffer primitives")
@@ -642,6 +690,8 @@ def main():
 
     if args.workload in LBFGS_WORKLOADS:
         return bench_lbfgs(args, pkg, dev)
+    if args.workload == "lm-ends":
+        return bench_lm_ends(args, pkg, dev)
     if args.workload == "primitives":
         return bench_primitives(args, pkg, dev)
     if args.workload == "placement":

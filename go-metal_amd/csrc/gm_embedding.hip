@@ -46,6 +46,7 @@ lookup_kernel(const T *table, const int *tokens, T *out, uint32_t rows, uint32_t
 // comparisons over the whole chip.  Longer lists are sorted in chunks; a token's place in the whole is then its
 // place in its chunk plus a binary search in every other one.
 constexpr int kSortChunk = 8192;
+constexpr int kMostTokens = 1 << 22;      // the merge's searches grow with the square of the list: 512 chunks are enough of them
 constexpr int kSortLanes = 16;        // lanes that share a part of the chunk; each compares kSortOwn tokens of its own with it
 constexpr int kSortOwn = 2;
 constexpr int kSortRows = kSortLanes * kSortOwn, kSortSlices = 64, kSortBlock = kSortLanes * kSortSlices;
@@ -396,7 +397,7 @@ try {
 
 uintptr_t gm_embedding_gradient_workspace(int num_tokens, int vocab_size, int dim)
 {
-    if (num_tokens < 0 || vocab_size <= 0 || dim <= 0) return 0;
+    if (num_tokens < 0 || num_tokens > kMostTokens || vocab_size <= 0 || dim <= 0) return 0;
     return gradient_space((size_t)num_tokens, (size_t)dim).bytes;
 }
 
@@ -414,6 +415,10 @@ try {
     if (int rc = embedding_arguments(token_buffer, rng_state, num_tokens, vocab_size, dim, output_gradient_stride,
                                      table_gradient_stride, dropout_probability, dropout_site, &d))
         return rc;
+    if (num_tokens > kMostTokens) {
+        set_error("a gradient of %d tokens: at most %d at a time (accumulate the parts)", num_tokens, kMostTokens);
+        return kRcRange;
+    }
     const size_t in = type_bytes(data_type), out = type_bytes(gradient_type);
     if (!element_aligned("output gradient", output_gradient_buffer, in) || !element_aligned("table gradient", table_gradient_buffer, out) ||
         !rows_fit("output gradient", output_gradient_buffer, (size_t)num_tokens, (size_t)dim, (size_t)output_gradient_stride, in) ||

@@ -449,7 +449,7 @@ int execute_embedding_lookup(uintptr_t device, uintptr_t command_queue, uintptr_
  * output gradients (through the same dropout) at every position that names v; fp32 sums, rounded once.  Tokens outside
  * the vocabulary and padding_token (-1: none) give nothing.  accumulate 0: every row is written, those that no token
  * names with zeros; otherwise the sums are added to what the buffer holds and other rows are not touched (gradient
- * accumulation, or a table tied to the output layer).  gradient_type: Float32, or data_type.
+ * accumulation, or a table tied to the output layer).  gradient_type: Float32, or data_type.  At most 2^22 tokens.
  * workspace: gm_embedding_gradient_workspace bytes, aligned to 256. */
 uintptr_t gm_embedding_gradient_workspace(int num_tokens, int vocab_size, int dim);
 int execute_embedding_gradient(uintptr_t device, uintptr_t command_queue, uintptr_t output_gradient_buffer,
