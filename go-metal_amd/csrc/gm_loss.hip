@@ -51,6 +51,14 @@ __device__ inline int chunk_rows(const LossHead *head, int first, int most)
 // ------------------------------------------------------------------------------------------ tokens that count ----
 constexpr int kScanBlock = 1024;
 
+__device__ inline void write_head(LossHead *head, int count, int mean, float gradient_scale, const AmpScaleView &amp)
+{
+    float scale = gradient_scale;
+    if (amp.scale[0]) scale = scale * *amp.scale[*amp.stamp[1] > *amp.stamp[0] ? 1 : 0];
+    head->count = count;
+    head->coefficient = mean ? scale / (float)(count > 0 ? count : 1) : scale;
+}
+
 // Packs the tokens that take part: row_of[r] is the r-th one, place_of[i] where token i went (-1: nowhere).
 __global__ void __launch_bounds__(kScanBlock)
 scan_targets_kernel(const int *targets, int n, int vocab, int ignore, int mean, float gradient_scale, AmpScaleView amp, LossHead *head,
@@ -85,12 +93,7 @@ scan_targets_kernel(const int *targets, int n, int vocab, int ignore, int mean, 
         done += of_wave[kScanBlock / 64];
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        float scale = gradient_scale;
-        if (amp.scale[0]) scale = scale * *amp.scale[*amp.stamp[1] > *amp.stamp[0] ? 1 : 0];
-        head->count = done;
-        head->coefficient = mean ? scale / (float)(done > 0 ? done : 1) : scale;
-    }
+    if (threadIdx.x == 0) write_head(head, done, mean, gradient_scale, amp);
 }
 
 // Eight elements as the planes of an operand: rounded to nearest, then what is left of them after that, and so on.
@@ -114,33 +117,77 @@ __device__ inline void load_padded(const I *row, int c, int dim, bool aligned, f
 
 constexpr int kPackBlock = 256;
 
+// Up to this many tokens every workgroup of pack_tokens_kernel counts the ones before its own by itself: a launch less, 2 to 3 us.
+constexpr int kCountedTokens = 2048;
+
+struct PackArgs {
+    int64_t x_stride, packed_stride, plane, dx_stride;
+    bool aligned;
+    int n, dim, width, planes;
+    // COUNT: what scan_targets_kernel does otherwise
+    const int *targets;
+    int vocab, ignore, mean;
+    float gradient_scale;
+    AmpScaleView amp;
+    int *row_of, *row_target;
+};
+
 // Workgroup i < n: token i's activations to their place, or zeros to its outputs.  The rows behind the last counted
 // token, up to a whole step of k, become zeros.
-template <typename I, typename T>
+template <typename I, typename T, bool COUNT>
 __global__ void __launch_bounds__(kPackBlock)
-pack_tokens_kernel(const I *x, int64_t x_stride, bool aligned, int n, int dim, int width, const LossHead *head, const int *place_of, T *packed,
-                   int64_t packed_stride, int64_t plane, int planes, float *losses, I *dx, int64_t dx_stride)
+pack_tokens_kernel(PackArgs a, const I *x, LossHead *head, const int *place_of, T *packed, float *losses, I *dx)
 {
+    __shared__ int of_wave[kPackBlock / 64];
     const int i = blockIdx.x;
-    if (i >= n) {
-        const int r = head->count + (i - n), end = (head->count + kStepK - 1) / kStepK * kStepK;
+    int place, count;
+    if (COUNT) {
+        // the counted tokens before i (all of them, for the workgroups behind the last token)
+        int mine = 0;
+        for (int j = threadIdx.x; j < (i < a.n ? i : a.n); j += kPackBlock) {
+            const int t = a.targets[j];
+            mine += t != a.ignore && (unsigned)t < (unsigned)a.vocab;
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o);
+        if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = mine;
+        __syncthreads();
+        place = 0;
+#pragma unroll
+        for (int w = 0; w < kPackBlock / 64; w++) place += of_wave[w];
+        count = place;
+        if (i == a.n && threadIdx.x == 0) write_head(head, count, a.mean, a.gradient_scale, a.amp);
+        if (i < a.n) {
+            const int t = a.targets[i];
+            if (t == a.ignore || (unsigned)t >= (unsigned)a.vocab) {
+                place = -1;
+            } else if (threadIdx.x == 0) {
+                a.row_of[place] = i;
+                a.row_target[place] = t;
+            }
+        }
+    } else {
+        place = i < a.n ? place_of[i] : -1;
+        count = head->count;
+    }
+    if (i >= a.n) {
+        const int r = count + (i - a.n), end = (count + kStepK - 1) / kStepK * kStepK;
         float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (r < end)
-            for (int c = threadIdx.x * 8; c < width; c += kPackBlock * 8) split_store<T>(zero, packed + r * packed_stride + c, plane, planes);
+            for (int c = threadIdx.x * 8; c < a.width; c += kPackBlock * 8) split_store<T>(zero, packed + r * a.packed_stride + c, a.plane, a.planes);
         return;
     }
-    const int place = place_of[i];
     if (place >= 0) {
-        for (int c = threadIdx.x * 8; c < width; c += kPackBlock * 8) {
+        for (int c = threadIdx.x * 8; c < a.width; c += kPackBlock * 8) {
             float v[8];
-            load_padded(x + (int64_t)i * x_stride, c, dim, aligned, v);
-            split_store<T>(v, packed + place * packed_stride + c, plane, planes);
+            load_padded(x + i * a.x_stride, c, a.dim, a.aligned, v);
+            split_store<T>(v, packed + place * a.packed_stride + c, a.plane, a.planes);
         }
         return;
     }
     if (threadIdx.x == 0) losses[i] = 0.0f;
     if (dx)
-        for (int c = threadIdx.x; c < dim; c += kPackBlock) dx[(int64_t)i * dx_stride + c] = (I)0.0f;
+        for (int c = threadIdx.x; c < a.dim; c += kPackBlock) dx[i * a.dx_stride + c] = (I)0.0f;
 }
 
 // The weights as operand rows of `width` elements (a multiple of 64), eight a lane.
@@ -329,7 +376,9 @@ rows_kernel(RowsArgs a)
     }
 }
 
-// The sum (or mean) of the losses and the number of tokens that count; one workgroup, sums in 64 bits in a fixed order.
+// The sum (or mean) of the losses and the number of tokens that count; one workgroup, sums in 64 bits in a fixed order.  (A launch
+// of its own: with the last of rows_kernel's workgroups doing it, the counting of all of them cost more, 3 us at 64 tokens
+// and 60 us at 4096.)
 __global__ void __launch_bounds__(1024)
 total_kernel(const float *losses, int n, int mean, const LossHead *head, float *loss)
 {
@@ -695,12 +744,18 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     const size_t rows = ((size_t)s.n + kStepK - 1) / kStepK * kStepK, chunk_rows = ((size_t)s.chunk + kStepK - 1) / kStepK * kStepK;
     const int64_t x_plane = (int64_t)rows * s.x_stride, w_plane = (int64_t)s.vocab * s.width, slope_plane = (int64_t)chunk_rows * s.slope_stride;
 
-    scan_targets_kernel<<<1, kScanBlock, 0, stream>>>(reinterpret_cast<const int *>(c.targets), s.n, s.vocab, c.ignore, c.mean,
-                                                      c.gradient_scale, c.amp, head, row_of, place_of, row_target);
-    pack_tokens_kernel<I, T><<<s.n + kStepK, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.hidden), c.hidden_stride,
-                                                                      c.hidden % 16 == 0 && c.hidden_stride * sizeof(I) % 16 == 0, s.n, s.dim,
-                                                                      s.width, head, place_of, x, s.x_stride, x_plane, s.planes, losses,
-                                                                      reinterpret_cast<I *>(c.dx), c.dx_stride);
+    const int *targets = reinterpret_cast<const int *>(c.targets);
+    const PackArgs pack{c.hidden_stride, s.x_stride, x_plane, c.dx_stride, c.hidden % 16 == 0 && c.hidden_stride * sizeof(I) % 16 == 0, s.n, s.dim, s.width,
+                        s.planes, targets, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, row_of, row_target};
+    const I *hidden = reinterpret_cast<const I *>(c.hidden);
+    I *dx = reinterpret_cast<I *>(c.dx);
+    if (s.n <= kCountedTokens) {
+        pack_tokens_kernel<I, T, true><<<s.n + kStepK, kPackBlock, 0, stream>>>(pack, hidden, head, place_of, x, losses, dx);
+    } else {
+        scan_targets_kernel<<<1, kScanBlock, 0, stream>>>(targets, s.n, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, head, row_of,
+                                                          place_of, row_target);
+        pack_tokens_kernel<I, T, false><<<s.n + kStepK, kPackBlock, 0, stream>>>(pack, hidden, head, place_of, x, losses, dx);
+    }
     Operand w{reinterpret_cast<const short *>(c.weight), c.weight_stride, 0, s.vocab};
     if (s.pack_weights) {
         const unsigned grid = (unsigned)(((int64_t)s.vocab * (s.width / 8) + kPackBlock - 1) / kPackBlock);
