@@ -25,6 +25,7 @@ namespace gm {
 struct LossHead {
     int count;                 // tokens that take part
     float coefficient;         // c above
+    int x_exponent, w_exponent;      // the largest of the rows' exponents (operands with a scale for each row)
 };
 
 typedef Shape<256, 256, 2, 4, 2> WideShape;       // products of many tiles: 128 KiB of LDS, one workgroup a CU
@@ -41,6 +42,16 @@ template <typename T>
 constexpr float kSlopeScale = 1.0f;
 template <>
 constexpr float kSlopeScale<_Float16> = 16384.0f;
+
+// Operands with a scale for each row.  fp32 tensors are multiplied as two parts of fp16 (h, and what is left of the value after
+// h) with the products h h, h l and l h: 22 bits and a bit, about what fp32 sums keep of the result.  fp16's short range is made up
+// for by the rows' own powers of two: a row whose largest element lies below 2^e is taken times 2^(15 - e), so that a part's
+// least step, 2^-24, is 2^-39 of the row's largest.  The logits' epilogue undoes both rows' powers.  Where a row's index is
+// what the sum runs over (W's in dX, X's in dW) its power goes into dS, relative to the largest row's; there are two sets of dS
+// then.  (Three parts of bfloat16 with six products need no scales, and took twice the matrix work: 513 x 10007 x 1000 in 293 us.)
+// bfloat16 activations are one such part, for a weight gradient in fp32: with dS in two parts that is two products, with
+// bfloat16 parts of dS it were three.
+constexpr int kRowBits = 15, kSlopeBits = 14;
 
 __device__ inline int chunk_rows(const LossHead *head, int first, int most)
 {
@@ -115,6 +126,39 @@ __device__ inline void load_padded(const I *row, int c, int dim, bool aligned, f
     load8(row + c, aligned && count == 8, count, v);
 }
 
+// The power of two of a row: its largest element lies below 2^e (0 for a row that is not finite; for a row of zeros less than any
+// other's, so that it takes no part in the largest).  One wavefront; the same in all lanes.
+template <typename I>
+__device__ inline int row_exponent(const I *row, int dim, bool aligned)
+{
+    const int lane = threadIdx.x & 63;
+    uint32_t top = 0;
+    for (int c = lane * 8; c < dim; c += 64 * 8) {
+        float v[8];
+        load_padded(row, c, dim, aligned, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t bits = __float_as_uint(v[e]) & 0x7FFFFFFFu;
+            top = top > bits ? top : bits;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const uint32_t other = (uint32_t)__shfl_xor((int)top, o);
+        top = top > other ? top : other;
+    }
+    if (top == 0) return -200;
+    int e = 0;
+    if (top < 0x7F800000u) (void)frexpf(__uint_as_float(top), &e);
+    return e;
+}
+
+__device__ inline void scale8(float (&v)[8], int e)
+{
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], e);
+}
+
 constexpr int kPackBlock = 256;
 
 // Up to this many tokens every workgroup of pack_tokens_kernel counts the ones before its own by itself: a launch less, 2 to 3 us.
@@ -130,6 +174,10 @@ struct PackArgs {
     float gradient_scale;
     AmpScaleView amp;
     int *row_of, *row_target;
+    // operand rows with a scale each
+    int scaled_planes;
+    _Float16 *scaled;
+    short *exponents;       // by packed token
 };
 
 // Workgroup i < n: token i's activations to their place, or zeros to its outputs.  The rows behind the last counted
@@ -174,14 +222,32 @@ pack_tokens_kernel(PackArgs a, const I *x, LossHead *head, const int *place_of, 
         const int r = count + (i - a.n), end = (count + kStepK - 1) / kStepK * kStepK;
         float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (r < end)
-            for (int c = threadIdx.x * 8; c < a.width; c += kPackBlock * 8) split_store<T>(zero, packed + r * a.packed_stride + c, a.plane, a.planes);
+            for (int c = threadIdx.x * 8; c < a.width; c += kPackBlock * 8) {
+                split_store<T>(zero, packed + r * a.packed_stride + c, a.plane, a.planes);
+                split_store<_Float16>(zero, a.scaled + r * a.packed_stride + c, a.plane, a.scaled_planes);
+            }
         return;
     }
     if (place >= 0) {
+        const I *row = x + i * a.x_stride;
+        int exponent = 0;
+        if (a.scaled_planes) {
+            exponent = row_exponent(row, a.dim, a.aligned);
+            if (threadIdx.x == 0) a.exponents[place] = (short)exponent;
+        }
         for (int c = threadIdx.x * 8; c < a.width; c += kPackBlock * 8) {
             float v[8];
-            load_padded(x + i * a.x_stride, c, a.dim, a.aligned, v);
-            split_store<T>(v, packed + place * a.packed_stride + c, a.plane, a.planes);
+            load_padded(row, c, a.dim, a.aligned, v);
+            if (a.planes) {
+                float copy[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) copy[e] = v[e];
+                split_store<T>(copy, packed + place * a.packed_stride + c, a.plane, a.planes);
+            }
+            if (a.scaled_planes) {
+                scale8(v, kRowBits - exponent);
+                split_store<_Float16>(v, a.scaled + place * a.packed_stride + c, a.plane, a.scaled_planes);
+            }
         }
         return;
     }
@@ -205,6 +271,54 @@ pack_weights_kernel(const I *w, int64_t w_stride, bool aligned, int rows, int di
     split_store<T>(v, packed + (int64_t)row * width + c, plane, planes);
 }
 
+// fp32 weights as two parts of fp16, a scale for each row; a wavefront a row.
+__global__ void __launch_bounds__(kPackBlock)
+pack_scaled_weights_kernel(const float *w, int64_t w_stride, bool aligned, int rows, int dim, int width, _Float16 *packed, int64_t plane,
+                           short *exponents)
+{
+    const int row = blockIdx.x * (kPackBlock / 64) + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const float *from = w + row * w_stride;
+    const int exponent = row_exponent(from, dim, aligned);
+    if ((threadIdx.x & 63) == 0) exponents[row] = (short)exponent;
+    for (int c = (threadIdx.x & 63) * 8; c < width; c += 64 * 8) {
+        float v[8];
+        load_padded(from, c, dim, aligned, v);
+        scale8(v, kRowBits - exponent);
+        split_store<_Float16>(v, packed + (int64_t)row * width + c, plane, 2);
+    }
+}
+
+// The largest of the rows' exponents; one workgroup.  (Every row's workgroup raising one word took 90 us for 10007 rows.)
+__global__ void __launch_bounds__(1024)
+largest_exponents_kernel(LossHead *head, const short *x, const short *w, int words)
+{
+    __shared__ int of_wave[2][16];
+    int top[2] = {-100000, -100000};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const short *from = k ? w : x;
+        const int n = k ? words : head->count;
+        for (int i = threadIdx.x * 8; i < n; i += 1024 * 8) {      // (the arrays are there in eights)
+            const s16x8 v = *reinterpret_cast<const s16x8 *>(from + i);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top[k] = i + e < n && v[e] > top[k] ? v[e] : top[k];
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            const int other = __shfl_xor(top[k], o);
+            top[k] = top[k] > other ? top[k] : other;
+        }
+        if ((threadIdx.x & 63) == 0) of_wave[k][threadIdx.x >> 6] = top[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        int most = -100000;
+        for (int wave = 0; wave < 16; wave++) most = most > of_wave[threadIdx.x][wave] ? most : of_wave[threadIdx.x][wave];
+        (threadIdx.x ? head->w_exponent : head->x_exponent) = most;
+    }
+}
+
 // --------------------------------------------------------------------------------------------------- logits ----
 enum : int { kKeepNothing, kKeepHalf, kKeepFloat };
 
@@ -219,6 +333,7 @@ struct LogitsArgs {
     int groups, keep;
     void *kept;                 // [row of the chunk][stride]
     int64_t stride;
+    const short *x_exponents, *w_exponents;      // nullptr: rows have no scales of their own.  Of w's, whole tiles are there
 };
 
 template <typename T, typename S>
@@ -243,6 +358,18 @@ logits_kernel(LogitsArgs a)
     const int wp = p0 + wave / S::WQ * (S::BP / S::WP) + (lane >> 4) * 4, wq = q0 + wave % S::WQ * (S::BQ / S::WQ) + (lane & 15);
     const int group = (p0 + wave / S::WQ * (S::BP / S::WP)) / (S::BP / S::WP);
     const bool ragged = p0 + S::BP > a.vocab;
+    if (a.w_exponents) {
+#pragma unroll
+        for (int j = 0; j < S::MQ; j++) {
+            const int by = (wq + j * 16 < rows ? a.x_exponents[a.first + wq + j * 16] : 0) - 2 * kRowBits;
+#pragma unroll
+            for (int i = 0; i < S::MP; i++) {
+                const s16x4 e = *reinterpret_cast<const s16x4 *>(a.w_exponents + wp + i * 16);
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[i][j][r] = ldexpf(acc[i][j][r], e[r] + by);
+            }
+        }
+    }
     // what this lane stores of the exponentials: always the same eight words
     const int wave_q = wq - (lane & 15), turn_col = wp - (lane >> 4) * 4 + lane % (64 / kTurnRows<S>) * 8;
     char *kept = static_cast<char *>(a.kept) + (wave_q * a.stride + turn_col) * (a.keep == kKeepFloat ? 4 : 2);
@@ -313,6 +440,10 @@ struct RowsArgs {
     int keep, planes;
     void *kept, *slopes;       // kKeepHalf: the same memory
     int64_t stride, plane;
+    // operands with scales: of w's rows for these slopes (nullptr: none), and a second set, for dW, with x's rows' (0 planes: none)
+    const short *w_exponents, *x_exponents;
+    int dw_planes;
+    _Float16 *dw_slopes;
 };
 
 __device__ inline float block_reduce(float x, bool maximum, float *scratch)
@@ -341,8 +472,10 @@ rows_kernel(RowsArgs a)
     const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (r >= rows) {
         if (a.keep != kKeepNothing && r < (rows + kStepK - 1) / kStepK * kStepK)      // a whole step of k for dW
-            for (int k = 0; k < a.planes; k++)
-                for (int c = threadIdx.x * 8; c < a.padded; c += kRowBlock * 8) store8(slopes + k * a.plane + c, true, 8, zero);
+            for (int c = threadIdx.x * 8; c < a.padded; c += kRowBlock * 8) {
+                for (int k = 0; k < a.planes; k++) store8(slopes + k * a.plane + c, true, 8, zero);
+                for (int k = 0; k < a.dw_planes; k++) store8(a.dw_slopes + r * a.stride + k * a.plane + c, true, 8, zero);
+            }
         return;
     }
     const float2 *stats = a.stats + (int64_t)r * a.groups;
@@ -357,6 +490,8 @@ rows_kernel(RowsArgs a)
     if (a.keep == kKeepNothing) return;
     const int target = a.row_target[a.first + r];
     const float at_target = expm1f(target_logit - lse);
+    const int w_shift = a.w_exponents ? kSlopeBits - a.head->w_exponent : 0;
+    const int x_shift = a.dw_planes ? a.x_exponents[a.first + r] - a.head->x_exponent + kSlopeBits : 0;
     for (int c = threadIdx.x * 8; c < a.padded; c += kRowBlock * 8) {
         float v[8];
         float f = c < a.vocab ? expf(stats[c / a.span].x - lse) : 0.0f;
@@ -367,12 +502,22 @@ rows_kernel(RowsArgs a)
             load8(static_cast<const float *>(a.kept) + r * a.stride + c, true, 8, v);
         }
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = c + e < a.vocab ? (c + e == target ? at_target : v[e] * f) * kSlopeScale<T> : 0.0f;
-        for (int k = 0; k < a.planes; k++) {
-            store8(slopes + k * a.plane + c, true, 8, v);
+        for (int e = 0; e < 8; e++) v[e] = c + e < a.vocab ? (c + e == target ? at_target : v[e] * f) : 0.0f;
+        if (a.dw_planes) {
+            float scaled[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = v[e] - (float)from_float<T>(v[e]);
+            for (int e = 0; e < 8; e++) scaled[e] = ldexpf(v[e], x_shift);
+            split_store<_Float16>(scaled, a.dw_slopes + r * a.stride + c, a.plane, a.dw_planes);
         }
+        if (a.w_exponents) {
+            const s16x8 e8 = *reinterpret_cast<const s16x8 *>(a.w_exponents + c);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = ldexpf(v[e], e8[e] + w_shift);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = v[e] * kSlopeScale<T>;
+        }
+        split_store<T>(v, slopes + c, a.plane, a.planes);
     }
 }
 
@@ -410,6 +555,7 @@ struct ProductArgs {
     const LossHead *head;
     const int *row_of;               // dX: where a packed row belongs
     float unscale;                   // undoes kSlopeScale
+    const int *exponent;             // of the largest row, where rows have scales (nullptr: they have none)
     void *out;
     int64_t out_stride;
     int out_type;
@@ -432,6 +578,13 @@ __device__ inline void finish_as(const ProductArgs &a, O *out, int64_t row, int 
         for (int e = 0; e < 8; e++) v[e] = old[e] + v[e];
     }
     store8(at, whole, count, v);
+}
+
+// What the sums are multiplied by.
+__device__ inline float output_factor(const ProductArgs &a)
+{
+    const float by = a.head->coefficient * a.unscale;
+    return a.exponent ? ldexpf(by, *a.exponent - kRowBits - kSlopeBits) : by;
 }
 
 // Eight outputs of one row: times c, added to what is there, rounded once.
@@ -541,7 +694,7 @@ product_kernel(ProductArgs a)
 #pragma unroll
             for (int j = 0; j < S::MQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    store_tile<S>(a, a.head->coefficient * a.unscale, p0, q0, split, product.turn_place(), acc);
+    store_tile<S>(a, output_factor(a), p0, q0, split, product.turn_place(), acc);
 }
 
 // The parts of a split sum, added up in order; eight outputs a lane.
@@ -569,7 +722,7 @@ join_splits_kernel(ProductArgs a)
                 for (int e = 0; e < 8; e++) sum[e] += v[k][e];
             }
     }
-    finish(a, a.head->coefficient * a.unscale, q, p, sum);
+    finish(a, output_factor(a), q, p, sum);
 }
 
 // ------------------------------------------------------------------------------------------------ host side ----
@@ -577,11 +730,11 @@ join_splits_kernel(ProductArgs a)
 struct LossPlan {
     int n, vocab, dim, width, padded, chunk, chunks;
     int x_stride, slope_stride;            // of the packed tokens and of dS
-    int operand_type;                      // kFloat16 or kBFloat16
-    int planes, slope_planes, keep;        // planes of x (and W); of dS
+    int planes, scaled_planes;             // planes of x (and of W, if it is packed) as it is; with a scale for each row
+    int slope_planes, dw_slope_planes, keep;      // of dS; of its second set, for dW
     bool gradients, pack_weights, sum_weights;      // sum_weights: dW of several chunks in 16 bits needs fp32 sums
     int logits_shape, groups, dx_shape, dx_splits, dw_shape, dw_splits;
-    size_t head, row_of, place_of, row_target, target_logit, x, w, stats, kept, slopes, partial, sums, bytes;
+    size_t head, row_of, place_of, row_target, target_logit, x, scaled_x, x_exponents, w, w_exponents, stats, kept, slopes, dw_slopes, partial, sums, bytes;
 };
 
 // Rows that the kernels lay out themselves are 128 bytes longer than their contents: a step reads 128 bytes of 256 rows, and
@@ -619,13 +772,14 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.n = n, s.vocab = vocab, s.dim = dim, s.gradients = gradients;
     s.width = (int)up((size_t)dim, kStepK), s.padded = (int)up((size_t)vocab, kStepK);
     s.x_stride = s.width + kSkew, s.slope_stride = s.padded + kSkew;
-    s.operand_type = data_type == kFloat32 ? kBFloat16 : data_type;
-    s.planes = data_type == kFloat32 ? 3 : 1;
-    // an fp32 gradient of 16-bit activations: as many parts of dS as leave nothing that fp32 sums would notice
-    s.slope_planes = gradient_type != kFloat32 ? 1 : data_type == kFloat16 ? 2 : 3;
-    s.keep = !gradients ? kKeepNothing : s.slope_planes == 1 ? kKeepHalf : kKeepFloat;
+    const bool exact = gradients && gradient_type == kFloat32;      // an fp32 weight gradient
+    s.planes = data_type == kFloat32 ? 0 : 1;
+    s.scaled_planes = data_type == kFloat32 ? 2 : data_type == kBFloat16 && exact ? 1 : 0;
+    s.slope_planes = data_type == kFloat32 || (data_type == kFloat16 && exact) ? 2 : 1;
+    s.dw_slope_planes = s.scaled_planes && gradients ? 2 : 0;
+    s.keep = !gradients ? kKeepNothing : exact ? kKeepFloat : kKeepHalf;
     s.pack_weights = data_type == kFloat32 || !weights_fit;
-    const size_t entry = s.keep == kKeepNothing ? 0 : s.keep == kKeepHalf ? 2 : 4 + 2 * s.slope_planes;
+    const size_t entry = s.keep == kKeepNothing ? 0 : s.keep == kKeepHalf ? 2 : 4 + 2 * (s.slope_planes + s.dw_slope_planes);
     if (chunk <= 0) {
         size_t most = entry ? kKeptBytes / (entry * s.slope_stride) / kLeastChunk * kLeastChunk : (size_t)n;
         if (most < kLeastChunk) most = kLeastChunk;
@@ -648,9 +802,9 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
             splits = parts(shape);
         };
         s.dx_shape = shape_for(dim, s.chunk);
-        split(s.dx_shape, s.dx_splits, dim, s.chunk, s.padded / kStepK * (s.planes == 3 ? 6 : 1));
+        split(s.dx_shape, s.dx_splits, dim, s.chunk, s.padded / kStepK * (s.scaled_planes == 2 ? 3 : 1));
         s.dw_shape = wide_or_square(dim, vocab);
-        split(s.dw_shape, s.dw_splits, dim, vocab, (s.chunk + kStepK - 1) / kStepK * (s.planes == 3 ? 6 : s.slope_planes));
+        split(s.dw_shape, s.dw_splits, dim, vocab, (s.chunk + kStepK - 1) / kStepK * (s.scaled_planes == 2 ? 3 : s.dw_slope_planes ? 2 : s.slope_planes));
     }
     const size_t rows = up((size_t)n, kStepK), chunk_rows = up((size_t)s.chunk, kStepK);
     size_t at = 0;
@@ -662,10 +816,14 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.head = take(sizeof(LossHead));
     s.row_of = take(4 * rows), s.place_of = take(4 * rows), s.row_target = take(4 * rows), s.target_logit = take(4 * rows);
     s.x = take(rows * s.x_stride * 2 * s.planes);
-    s.w = take(s.pack_weights ? (size_t)vocab * s.width * 2 * s.planes : 0);
+    s.scaled_x = take(rows * s.x_stride * 2 * s.scaled_planes);
+    s.x_exponents = take(s.scaled_planes ? 2 * rows : 0);
+    s.w = take(s.pack_weights ? (size_t)vocab * s.width * 2 * (data_type == kFloat32 ? 2 : 1) : 0);
+    s.w_exponents = take(data_type == kFloat32 ? 2 * up((size_t)vocab, 256) : 0);      // whole tiles of words
     s.stats = take(sizeof(float2) * (size_t)s.chunk * s.groups);
     s.kept = take(s.keep == kKeepNothing ? 0 : chunk_rows * s.slope_stride * (s.keep == kKeepHalf ? 2 : 4));
     s.slopes = s.keep == kKeepFloat ? take(chunk_rows * s.slope_stride * 2 * s.slope_planes) : s.kept;
+    s.dw_slopes = take(chunk_rows * s.slope_stride * 2 * s.dw_slope_planes);
     // (dX is joined before dW's parts are written)
     const size_t dx_parts = gradients && s.dx_splits > 1 ? (size_t)s.dx_splits * s.chunk * dim * 4 : 0;
     const size_t dw_parts = gradients && s.dw_splits > 1 ? (size_t)s.dw_splits * vocab * dim * 4 : 0;
@@ -692,12 +850,10 @@ static bool weights_fit(uintptr_t weight, int dim, int stride, int data_type)
     return data_type != kFloat32 && weight != 0 && weight % 16 == 0 && dim % kStepK == 0 && stride % 8 == 0 && stride <= 1 << 22;
 }
 
+// Codes: P plane + 4 Q plane; the small products first.
 static constexpr PlanePairs kOnePair = {1, 0x0};
-// fp32 by three planes of eight bits: the six products of 2^-16 and more, the small ones first
-// (codes: P plane + 4 Q plane)
-static constexpr PlanePairs kSixPairs = {6, 0x041528};
-// x (one plane) with the parts of dS: the smallest first
-static constexpr PlanePairs kTwoSlopes = {2, 0x04}, kThreeSlopes = {3, 0x048};
+static constexpr PlanePairs kBothParts = {3, 0x041};      // l h, h l, h h
+static constexpr PlanePairs kPartsOfQ = {2, 0x04};        // h l, h h where P has one plane
 
 struct LossCall {
     uintptr_t hidden, weight, targets, losses, loss, dx, dw;
@@ -744,9 +900,13 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     const size_t rows = ((size_t)s.n + kStepK - 1) / kStepK * kStepK, chunk_rows = ((size_t)s.chunk + kStepK - 1) / kStepK * kStepK;
     const int64_t x_plane = (int64_t)rows * s.x_stride, w_plane = (int64_t)s.vocab * s.width, slope_plane = (int64_t)chunk_rows * s.slope_stride;
 
+    _Float16 *scaled_x = reinterpret_cast<_Float16 *>(space + s.scaled_x);
+    short *x_exponents = reinterpret_cast<short *>(space + s.x_exponents), *w_exponents = reinterpret_cast<short *>(space + s.w_exponents);
+    constexpr bool kFull = std::is_same<I, float>::value;      // fp32: every operand has scales
     const int *targets = reinterpret_cast<const int *>(c.targets);
     const PackArgs pack{c.hidden_stride, s.x_stride, x_plane, c.dx_stride, c.hidden % 16 == 0 && c.hidden_stride * sizeof(I) % 16 == 0, s.n, s.dim, s.width,
-                        s.planes, targets, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, row_of, row_target};
+                        s.planes, targets, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, row_of, row_target, s.scaled_planes, scaled_x,
+                        x_exponents};
     const I *hidden = reinterpret_cast<const I *>(c.hidden);
     I *dx = reinterpret_cast<I *>(c.dx);
     if (s.n <= kCountedTokens) {
@@ -757,24 +917,32 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
         pack_tokens_kernel<I, T, false><<<s.n + kStepK, kPackBlock, 0, stream>>>(pack, hidden, head, place_of, x, losses, dx);
     }
     Operand w{reinterpret_cast<const short *>(c.weight), c.weight_stride, 0, s.vocab};
-    if (s.pack_weights) {
+    const bool w_aligned = c.weight % 16 == 0 && c.weight_stride * sizeof(I) % 16 == 0;
+    if constexpr (kFull) {
+        pack_scaled_weights_kernel<<<(s.vocab + kPackBlock / 64 - 1) / (kPackBlock / 64), kPackBlock, 0, stream>>>(
+            reinterpret_cast<const float *>(c.weight), c.weight_stride, w_aligned, s.vocab, s.dim, s.width,
+            reinterpret_cast<_Float16 *>(space + s.w), w_plane, w_exponents);
+    } else if (s.pack_weights) {
         const unsigned grid = (unsigned)(((int64_t)s.vocab * (s.width / 8) + kPackBlock - 1) / kPackBlock);
-        pack_weights_kernel<I, T><<<grid, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight), c.weight_stride,
-                                                                   c.weight % 16 == 0 && c.weight_stride * sizeof(I) % 16 == 0, s.vocab, s.dim,
+        pack_weights_kernel<I, T><<<grid, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight), c.weight_stride, w_aligned, s.vocab, s.dim,
                                                                    s.width, reinterpret_cast<T *>(space + s.w), w_plane, s.planes);
-        w = Operand{reinterpret_cast<const short *>(space + s.w), s.width, w_plane, s.vocab};
     }
-    const PlanePairs pairs = s.planes == 3 ? kSixPairs : kOnePair;
+    if (s.dw_slope_planes) largest_exponents_kernel<<<1, 1024, 0, stream>>>(head, x_exponents, w_exponents, kFull ? s.vocab : 0);
+    if (s.pack_weights) w = Operand{reinterpret_cast<const short *>(space + s.w), s.width, w_plane, s.vocab};
+    const PlanePairs pairs = kFull ? kBothParts : kOnePair;
     for (int k = 0; k < s.chunks; k++) {
         const int first = k * s.chunk, most = s.n - first < s.chunk ? s.n - first : s.chunk;
         if (most <= 0 && k > 0) break;
-        const Operand xs{reinterpret_cast<const short *>(x + (int64_t)first * s.x_stride), s.x_stride, x_plane, 0};
+        const Operand plain{reinterpret_cast<const short *>(x + (int64_t)first * s.x_stride), s.x_stride, x_plane, 0};
+        const Operand scaled{reinterpret_cast<const short *>(scaled_x + (int64_t)first * s.x_stride), s.x_stride, x_plane, 0};
         const int tokens = most > 0 ? most : 0;
-        LogitsArgs l{w, xs, pairs, s.width / kStepK, first, tokens, s.vocab, s.padded, head, row_target, target_logit,
-                     reinterpret_cast<float2 *>(space + s.stats), s.groups, s.keep, space + s.kept, s.slope_stride};
+        LogitsArgs l{w, kFull ? scaled : plain, pairs, s.width / kStepK, first, tokens, s.vocab, s.padded, head, row_target, target_logit,
+                     reinterpret_cast<float2 *>(space + s.stats), s.groups, s.keep, space + s.kept, s.slope_stride, kFull ? x_exponents : nullptr,
+                     kFull ? w_exponents : nullptr};
         RowsArgs r{first, tokens, s.vocab, s.padded, s.groups, kShapeSpan[s.logits_shape], head, row_of, row_target, target_logit,
                    reinterpret_cast<const float2 *>(space + s.stats), losses, s.keep, s.slope_planes, space + s.kept, space + s.slopes,
-                   s.slope_stride, slope_plane};
+                   s.slope_stride, slope_plane, kFull ? w_exponents : nullptr, x_exponents, s.dw_slope_planes,
+                   reinterpret_cast<_Float16 *>(space + s.dw_slopes)};
         if (tokens > 0) {
             launch_logits<T>(s.logits_shape, l, tokens, stream);
             rows_kernel<T><<<(tokens + kStepK - 1) / kStepK * kStepK, kRowBlock, 0, stream>>>(r);
@@ -786,16 +954,19 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
             a.p = w, a.p.rows = s.dim, a.q = slopes, a.pairs = pairs;
             a.first = first, a.most = tokens, a.steps = s.padded / kStepK, a.limit_p = s.vocab;
             a.splits = s.dx_splits, a.partial = reinterpret_cast<float *>(space + s.partial), a.partial_rows = tokens;
-            a.head = head, a.row_of = row_of, a.unscale = 1.0f / kSlopeScale<T>;
+            a.head = head, a.row_of = row_of, a.unscale = kFull ? 1.0f : 1.0f / kSlopeScale<T>, a.exponent = kFull ? &head->w_exponent : nullptr;
             a.out = reinterpret_cast<void *>(c.dx), a.out_stride = c.dx_stride, a.out_type = c.data_type;
             a.out_aligned = c.dx % 16 == 0 && c.dx_stride * sizeof(I) % 16 == 0;
             launch_product<T, false>(s.dx_shape, a, s.dim, tokens, stream);
         }
         if (c.dw) {
             ProductArgs a{};
-            a.p = xs, a.p.rows = s.dim, a.q = slopes, a.q.rows = s.vocab;
-            a.pairs = s.planes == 3 ? kSixPairs : s.slope_planes == 3 ? kThreeSlopes : s.slope_planes == 2 ? kTwoSlopes : kOnePair;
-            a.first = first, a.most = tokens, a.head = head, a.unscale = 1.0f / kSlopeScale<T>;
+            const bool scales = s.dw_slope_planes != 0;
+            a.p = scales ? scaled : plain, a.p.rows = s.dim;
+            a.q = scales ? Operand{reinterpret_cast<const short *>(space + s.dw_slopes), s.slope_stride, slope_plane, 0} : slopes, a.q.rows = s.vocab;
+            a.pairs = kFull ? kBothParts : scales || s.slope_planes == 2 ? kPartsOfQ : kOnePair;
+            a.first = first, a.most = tokens, a.head = head, a.unscale = scales ? 1.0f : 1.0f / kSlopeScale<T>;
+            a.exponent = scales ? &head->x_exponent : nullptr;
             a.splits = s.dw_splits, a.partial = reinterpret_cast<float *>(space + s.partial), a.partial_rows = s.vocab;
             const bool last = k + 1 == s.chunks;
             float *sums = reinterpret_cast<float *>(space + s.sums);
@@ -809,7 +980,8 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
                 a.add = s.sum_weights && k > 0 ? sums : nullptr;
             }
             a.skip_empty = a.accumulate && !a.add;
-            launch_product<T, true>(s.dw_shape, a, s.dim, s.vocab, stream);
+            if (scales) launch_product<_Float16, true>(s.dw_shape, a, s.dim, s.vocab, stream);
+            else launch_product<T, true>(s.dw_shape, a, s.dim, s.vocab, stream);
         }
     }
     total_kernel<<<1, 1024, 0, stream>>>(losses, s.n, c.mean, head, reinterpret_cast<float *>(c.loss));
@@ -891,7 +1063,7 @@ try {
     if (amp_state != 0 && !amp_scale_view(amp_state, ctx, &c.amp)) return kRcAmp;
     DeviceScope scope(ctx);
     if (!scope.ok()) return kRcHip;
-    if (data_type == kFloat32) launch_loss<float, __bf16>(c, plan, stream);
+    if (data_type == kFloat32) launch_loss<float, _Float16>(c, plan, stream);
     else if (data_type == kFloat16) launch_loss<_Float16, _Float16>(c, plan, stream);
     else launch_loss<__bf16, __bf16>(c, plan, stream);
     return hip_ok(hipGetLastError(), "linear cross entropy launch") ? 0 : kRcHip;

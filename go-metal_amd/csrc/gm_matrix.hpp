@@ -7,8 +7,8 @@
 // so no operand is ever copied to turn it.  P is the matrix instruction's first operand: a lane then holds four
 // consecutive p of one q, and outputs are stored along p.
 //
-// An fp32 operand comes as planes of bfloat16 (each the rounded rest of those before it); the sum then runs over
-// pairs of planes as well.  16-bit operands have one plane and one pair.
+// An operand of more bits comes as planes (each the rounded rest of those before it); the sum then runs over pairs of planes
+// as well.  16-bit operands have one plane and one pair.
 #pragma once
 
 #include "gm_ops.hpp"

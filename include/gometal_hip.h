@@ -469,9 +469,10 @@ int execute_embedding_gradient(uintptr_t device, uintptr_t command_queue, uintpt
  *               read on the device when the call runs.  Either handle may be 0; both: the loss alone.  A gradient that
  *               overflows its type is +-inf, which the mixed-precision step drops.
  *   accumulate: the weight gradient is added to what its buffer holds.
- * With a Float32 gradient_type the slope of the softmax is carried in 16-bit parts (two of Float16, three of BFloat16:
- * 22 bits and more); with a 16-bit one it is rounded to that type once.  Float32 tensors are multiplied as three bfloat16 parts each, with
- * products down to 2^-16 of the largest: about fp32's own accuracy for values below 3.3e38.
+ * With a Float32 gradient_type the slope of the softmax is carried in two parts of Float16 (22 bits); with a 16-bit one it is
+ * rounded to that type once.  Float32 tensors are multiplied as two parts of Float16, each row scaled by a power of two, with
+ * products down to 2^-22 of the largest: about the accuracy of fp32 sums; an element below 2^-18 of its row's largest keeps
+ * fewer bits (its error stays below 2^-40 of the row's largest, and the slope's below 2^-39).
  * workspace: gm_linear_cross_entropy_workspace bytes are enough for the fastest form; anything from
  * gm_linear_cross_entropy_least_workspace on works, with fewer tokens at a time.  Aligned to 256.  Both take the weight's
  * handle and stride because rows that the kernels can take as they lie (16-bit, dim a multiple of 64, stride of 8, base

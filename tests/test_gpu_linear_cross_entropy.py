@@ -1,12 +1,15 @@
 """The linear cross entropy against its formula in 64 bits.
 
 Bounds, in half steps u = 2^-24 of fp32.  A logit is a sum of D exact products in fp32: its error is at most
-delta = (D + 8) u sum |x w| (fp32 operands in parts: what the six products leave out is below 8 u of the same sum).  An
+delta = (D + 8) u sum |x w|.  fp32 operands are two parts of fp16, the second rounded to 2^-22 of the element or, with
+the row's largest below 2^e, 2^(e - 40), whichever is more; that, for both operands, and the product of the second parts, 2^-22 again,
+are 12 u of the same sum more, and 2^(e - 40) of each operand's row with the other's magnitudes.  An
 exponential's relative error is its argument's, (|s| u) for the difference and as much for the change of base, and a few
 u of its own; the sum over the vocabulary adds at most 200 u (no lane adds more than 128 terms in a row, trees the rest).
 So a loss is off by at most 2 delta + (4 R + 210) u + 2 u |lse|, R the largest |s - max|.  An entry p of the softmax is off by that much relative to p, plus
 what rounding takes: twice the half step of fp16 where exponentials are kept in it, and the half step of the type the
-slope is carried in.  The products sum V (or N) terms in fp32, and the result is rounded once."""
+slope is carried in; as two parts of fp16, 2^-22.  The products sum V (or N) terms in fp32, and the result is rounded once.
+Where the slope's parts carry a row's power of two their least error is 2^-39 of the largest row's other operand."""
 import numpy as np
 import pytest
 
@@ -55,7 +58,10 @@ def check(got, t, o, x, w, targets, mean=1, scale=1.0, add=None):
     fx = np.where(counts[:, None], fx, 0.0)
     s = fx @ fw.T
     top = s.max(1, keepdims=True)
-    delta = (d + 8) * U * (np.abs(fx) @ np.abs(fw).T).max(1)
+    delta = (d + (20 if t == F32 else 8)) * U * (np.abs(fx) @ np.abs(fw).T).max(1)
+    reach = lambda m: 2 * np.abs(m).max(initial=0.0)      # of 2^e, over all rows
+    if t == F32:
+        delta = delta + 2.0 ** -40 * (reach(fx) * np.abs(fw).sum(1).max() + reach(fw) * np.abs(fx).sum(1))
     off = 2 * delta + (4 * (top - s).max(1) + 210) * U + 2 * U * np.abs(top[:, 0] + np.log(v))      # per token
     assert np.all(np.abs(got["losses"] - losses) <= np.where(counts, off, 0.0))
     assert got["loss"][1] == count
@@ -65,17 +71,18 @@ def check(got, t, o, x, w, targets, mean=1, scale=1.0, add=None):
     p = np.clip(p, 0, 1)
     kept = 2 * HALF_STEP[F16] if o != F32 else 0.0
     # least values: fp16 keeps exponentials down to 2^-39 of their tile's largest and slopes down to 2^-38
-    floor = 2.0 ** -37 if o != F32 else 2.0 ** -100
+    floor = 2.0 ** -37 if t != F32 else 0.0
     for name, kind, value, right, over in (("dx", t, dx, lambda a: a @ np.abs(fw), v), ("dw", o, dw, lambda a: a.T @ np.abs(fx), n)):
         if name not in got:
             continue
-        slope = HALF_STEP[t] if name == "dx" or o != F32 or t == F32 else HALF_STEP[t] ** 2
-        if t == F32:
-            slope = 2.0 ** -22      # three parts
-        err = np.where(counts[:, None], p * (off[:, None] + (kept + 4 * U) * (ds > 0)) + np.abs(ds) * (slope + (over + 10) * U) + floor, 0.0)
+        parts = t == F32 or (name == "dw" and o == F32)
+        slope = 2.0 ** -22 if parts else HALF_STEP[t]
+        err = np.where(counts[:, None], p * (off[:, None] + (kept + 4 * U) * (ds > 0)) + np.abs(ds) * (slope + (over + 22) * U) + floor, 0.0)
         if name == "dw" and add is not None:
             value = value + to_float(add, o)
-        bound = c * right(err) + HALF_STEP[kind] * np.abs(value) * (1 + 2.0 ** -7) + TINY[kind] + 4 * U * np.abs(value)
+        other = fw if name == "dx" else fx
+        least = (over * 2.0 ** -39 + np.abs(ds).sum(1 if name == "dx" else 0)[:, None] * 2.0 ** -40) * reach(other) if parts else 0.0
+        bound = c * (right(err) + least) + HALF_STEP[kind] * np.abs(value) * (1 + 2.0 ** -7) + TINY[kind] + 4 * U * np.abs(value)
         diff = np.abs(to_float(got[name], kind).astype(np.float64) - value)
         assert np.all(diff <= bound), (name, (diff / bound).max())
 
@@ -209,6 +216,22 @@ def test_certain_and_hopeless_tokens(t):
     x = to_bits(lean[:, None] * to_float(w, t)[targets], t)
     with Buffers() as b:
         check(run(b, t, t, x, w, targets, scale=16.0), t, t, x, w, targets, scale=16.0)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_rows_of_very_different_size(t):
+    """Rows of both operands between 2^-40 and 2^20 times the others (and rows of zeros): the rows' powers of two are undone
+    exactly, and what a sum leaves out of a small row stays below its largest term's error."""
+    n, v, d = 70, 200, 96
+    x, w, targets = data(t, n, v, d)
+    rng = np.random.default_rng(12)
+    fx = to_float(x, t) * np.exp2(rng.integers(-40, 3, (n, 1))).astype(np.float32)
+    fw = to_float(w, t) * np.exp2(rng.integers(-40, 3, (v, 1))).astype(np.float32)
+    fx[5], fw[7] = 0.0, 0.0
+    small = to_bits(fx * np.float32(2.0 ** 20), t), to_bits(fw * np.float32(2.0 ** -20), t)
+    for x, w in ((to_bits(fx, t), to_bits(fw, t)), small):
+        with Buffers() as b:
+            check(run(b, t, F32, x, w, targets, scale=4.0), t, F32, x, w, targets, scale=4.0)
 
 
 def test_overflow_is_inf_and_nan_spreads_as_in_the_formula():

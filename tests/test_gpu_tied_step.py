@@ -64,7 +64,8 @@ def formula(table, tokens, targets, state, t=F32, move=None):
 
     r is half a step of the type that tensors are stored in, u of fp32, in which sums are made.  h is rounded twice on its way (and
     made by three products in fp32); a logit is off by what that does to it and by (D + 8) u of its terms' magnitudes (D); a
-    softmax entry p by that, twice, by the exponential's (4 R + 210) u and (16-bit types) by 3 r, and the slope by r more.  Every
+    softmax entry p by that, twice, by the exponential's (4 R + 210) u and (16-bit types) by 3 r, and the slope by r more (fp32: operands and slopes are two parts of fp16,
+    12 u a product more and 4 u for the slope).  Every
     gradient that is stored is rounded once, the table's a second time when the lookup's is added."""
     v, d = table.shape
     n = tokens.size
@@ -87,9 +88,10 @@ def formula(table, tokens, targets, state, t=F32, move=None):
     ds = p.copy()
     ds[at] -= 1.0
     err_h = np.abs(h) * (2 * r + 4 * u)
-    delta = (err_h[rows] @ np.abs(e).T + (d + 8) * u * (np.abs(h[rows]) @ np.abs(e).T)).max(1)
+    # (what the parts' least steps, 2^-40 and 2^-39 of a row's largest, add is below the 1 % that errors are taken larger at the end)
+    delta = (err_h[rows] @ np.abs(e).T + (d + (8 if t != F32 else 20)) * u * (np.abs(h[rows]) @ np.abs(e).T)).max(1)
     off = 2 * delta + (4 * (top - s).max(1) + 210) * u + 2 * u * np.abs(top[:, 0] + np.log(v))
-    err_ds = p * (off[:, None] + 3 * r) + np.abs(ds) * (r + 10 * u) + (2.0 ** -37 if t != F32 else 0.0)
+    err_ds = p * (off[:, None] + 3 * r) + np.abs(ds) * (r + 30 * u) + (2.0 ** -37 if t != F32 else 0.0)
     grad = c * (ds.T @ h[rows])
     err = c * (err_ds.T @ np.abs(h[rows]) + np.abs(ds).T @ err_h[rows] + n * u * (np.abs(ds).T @ np.abs(h[rows]))) + r * np.abs(grad)
     back, err_back = np.zeros((n, d)), np.zeros((n, d))
