@@ -36,7 +36,7 @@ enum : int { kWide, kSquare, kTall, kFlat };
 constexpr int kShapeP[4] = {256, 128, 256, 128}, kShapeQ[4] = {256, 128, 128, 32}, kShapeSpan[4] = {128, 64, 64, 32};
 
 // exp(s - m) in 16 bits is 32768 times itself in fp16, dS of fp16 operands 16384 times itself: both keep clear of the
-// subnormals (down to 2^-29 and 2^-28), and an entry's rounding is 2^-12 of it.
+// subnormals (down to 2^-29 and 2^-28), and an entry's rounding is at most 2^-11 of it.
 constexpr float kExpScale = 32768.0f, kExpShift = 15.0f;
 template <typename T>
 constexpr float kSlopeScale = 1.0f;
@@ -165,9 +165,10 @@ constexpr int kPackBlock = 256;
 constexpr int kCountedTokens = 2048;
 
 struct PackArgs {
-    int64_t x_stride, packed_stride, plane, dx_stride;
+    int64_t x_stride, packed_stride, plane, dx_stride;      // plane: of the scaled rows
     bool aligned;
-    int n, dim, width, planes;
+    int n, dim, width;
+    bool plain;             // the rows as they are
     // COUNT: what scan_targets_kernel does otherwise
     const int *targets;
     int vocab, ignore, mean;
@@ -223,7 +224,7 @@ pack_tokens_kernel(PackArgs a, const I *x, LossHead *head, const int *place_of, 
         float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (r < end)
             for (int c = threadIdx.x * 8; c < a.width; c += kPackBlock * 8) {
-                split_store<T>(zero, packed + r * a.packed_stride + c, a.plane, a.planes);
+                if (a.plain) store8(packed + r * a.packed_stride + c, true, 8, zero);
                 split_store<_Float16>(zero, a.scaled + r * a.packed_stride + c, a.plane, a.scaled_planes);
             }
         return;
@@ -238,12 +239,7 @@ pack_tokens_kernel(PackArgs a, const I *x, LossHead *head, const int *place_of, 
         for (int c = threadIdx.x * 8; c < a.width; c += kPackBlock * 8) {
             float v[8];
             load_padded(row, c, a.dim, a.aligned, v);
-            if (a.planes) {
-                float copy[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) copy[e] = v[e];
-                split_store<T>(copy, packed + place * a.packed_stride + c, a.plane, a.planes);
-            }
+            if (a.plain) store8(packed + place * a.packed_stride + c, true, 8, v);
             if (a.scaled_planes) {
                 scale8(v, kRowBits - exponent);
                 split_store<_Float16>(v, a.scaled + place * a.packed_stride + c, a.plane, a.scaled_planes);
@@ -259,7 +255,7 @@ pack_tokens_kernel(PackArgs a, const I *x, LossHead *head, const int *place_of, 
 // The weights as operand rows of `width` elements (a multiple of 64), eight a lane.
 template <typename I, typename T>
 __global__ void __launch_bounds__(kPackBlock)
-pack_weights_kernel(const I *w, int64_t w_stride, bool aligned, int rows, int dim, int width, T *packed, int64_t plane, int planes)
+pack_weights_kernel(const I *w, int64_t w_stride, bool aligned, int rows, int dim, int width, T *packed)
 {
     const int per_row = width / 8;
     const int64_t first = (int64_t)blockIdx.x * kPackBlock;
@@ -268,7 +264,7 @@ pack_weights_kernel(const I *w, int64_t w_stride, bool aligned, int rows, int di
     if (row >= rows) return;
     float v[8];
     load_padded(w + row * w_stride, c, dim, aligned, v);
-    split_store<T>(v, packed + (int64_t)row * width + c, plane, planes);
+    store8(packed + (int64_t)row * width + c, true, 8, v);
 }
 
 // fp32 weights as two parts of fp16, a scale for each row; a wavefront a row.
@@ -349,7 +345,8 @@ logits_kernel(LogitsArgs a)
     f32x4 acc[S::MP][S::MQ];
     const uint32_t lds = (uint32_t)(uintptr_t)(GM_LDS char *)tiles;
     // One tile of tokens: nobody shares the weights' rows, and every workgroup begins at a k of its own.  At one k the rows of all
-    // tiles, a power of two apart, lie on one channel: 1.07 GB of weights pass at 6.2 TB/s instead of 5.
+    // tiles, a power of two apart, lie on one channel: 128 x 65536 x 4096, 537 MB of weights, 165 -> 135 us.  (Up to 32 tokens,
+    // where tiles are half as high and four steps are in flight, it gains nothing: 203 -> 207 us for one token.)
     const int first = rows <= S::BQ && S::BQ > 32 ? (int)(tp * 5 % (uint32_t)a.steps) : 0;
     Multiplier<T, S, false, false> product(a.w, a.x, a.pairs, a.steps, 0, 0, first, first + a.steps * a.pairs.count, lds);
     product.start(p0, q0);
@@ -730,7 +727,8 @@ join_splits_kernel(ProductArgs a)
 struct LossPlan {
     int n, vocab, dim, width, padded, chunk, chunks;
     int x_stride, slope_stride;            // of the packed tokens and of dS
-    int planes, scaled_planes;             // planes of x (and of W, if it is packed) as it is; with a scale for each row
+    bool plain;                            // x (and W, if it is packed) as it is
+    int scaled_planes;                     // and with a scale for each row
     int slope_planes, dw_slope_planes, keep;      // of dS; of its second set, for dW
     bool gradients, pack_weights, sum_weights;      // sum_weights: dW of several chunks in 16 bits needs fp32 sums
     int logits_shape, groups, dx_shape, dx_splits, dw_shape, dw_splits;
@@ -740,7 +738,6 @@ struct LossPlan {
 // Rows that the kernels lay out themselves are 128 bytes longer than their contents: a step reads 128 bytes of 256 rows, and
 // rows a large power of two apart would all lie on the same channel of the L2.
 constexpr int kSkew = 64;
-
 
 constexpr int kLeastChunk = 256;
 constexpr size_t kKeptBytes = (size_t)4 << 30;      // of exp(s - m) and dS together, unless one chunk needs more
@@ -773,7 +770,7 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.width = (int)up((size_t)dim, kStepK), s.padded = (int)up((size_t)vocab, kStepK);
     s.x_stride = s.width + kSkew, s.slope_stride = s.padded + kSkew;
     const bool exact = gradients && gradient_type == kFloat32;      // an fp32 weight gradient
-    s.planes = data_type == kFloat32 ? 0 : 1;
+    s.plain = data_type != kFloat32;
     s.scaled_planes = data_type == kFloat32 ? 2 : data_type == kBFloat16 && exact ? 1 : 0;
     s.slope_planes = data_type == kFloat32 || (data_type == kFloat16 && exact) ? 2 : 1;
     s.dw_slope_planes = s.scaled_planes && gradients ? 2 : 0;
@@ -815,7 +812,7 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     };
     s.head = take(sizeof(LossHead));
     s.row_of = take(4 * rows), s.place_of = take(4 * rows), s.row_target = take(4 * rows), s.target_logit = take(4 * rows);
-    s.x = take(rows * s.x_stride * 2 * s.planes);
+    s.x = take(s.plain ? rows * s.x_stride * 2 : 0);
     s.scaled_x = take(rows * s.x_stride * 2 * s.scaled_planes);
     s.x_exponents = take(s.scaled_planes ? 2 * rows : 0);
     s.w = take(s.pack_weights ? (size_t)vocab * s.width * 2 * (data_type == kFloat32 ? 2 : 1) : 0);
@@ -905,7 +902,7 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     constexpr bool kFull = std::is_same<I, float>::value;      // fp32: every operand has scales
     const int *targets = reinterpret_cast<const int *>(c.targets);
     const PackArgs pack{c.hidden_stride, s.x_stride, x_plane, c.dx_stride, c.hidden % 16 == 0 && c.hidden_stride * sizeof(I) % 16 == 0, s.n, s.dim, s.width,
-                        s.planes, targets, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, row_of, row_target, s.scaled_planes, scaled_x,
+                        s.plain, targets, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, row_of, row_target, s.scaled_planes, scaled_x,
                         x_exponents};
     const I *hidden = reinterpret_cast<const I *>(c.hidden);
     I *dx = reinterpret_cast<I *>(c.dx);
@@ -925,7 +922,7 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     } else if (s.pack_weights) {
         const unsigned grid = (unsigned)(((int64_t)s.vocab * (s.width / 8) + kPackBlock - 1) / kPackBlock);
         pack_weights_kernel<I, T><<<grid, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight), c.weight_stride, w_aligned, s.vocab, s.dim,
-                                                                   s.width, reinterpret_cast<T *>(space + s.w), w_plane, s.planes);
+                                                                   s.width, reinterpret_cast<T *>(space + s.w));
     }
     if (s.dw_slope_planes) largest_exponents_kernel<<<1, 1024, 0, stream>>>(head, x_exponents, w_exponents, kFull ? s.vocab : 0);
     if (s.pack_weights) w = Operand{reinterpret_cast<const short *>(space + s.w), s.width, w_plane, s.vocab};
@@ -941,7 +938,7 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
                      kFull ? w_exponents : nullptr};
         RowsArgs r{first, tokens, s.vocab, s.padded, s.groups, kShapeSpan[s.logits_shape], head, row_of, row_target, target_logit,
                    reinterpret_cast<const float2 *>(space + s.stats), losses, s.keep, s.slope_planes, space + s.kept, space + s.slopes,
-                   s.slope_stride, slope_plane, kFull ? w_exponents : nullptr, x_exponents, s.dw_slope_planes,
+                   s.slope_stride, slope_plane, kFull ? w_exponents : nullptr, x_exponents, c.dw ? s.dw_slope_planes : 0,
                    reinterpret_cast<_Float16 *>(space + s.dw_slopes)};
         if (tokens > 0) {
             launch_logits<T>(s.logits_shape, l, tokens, stream);

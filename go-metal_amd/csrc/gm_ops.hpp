@@ -61,16 +61,6 @@ inline bool element_aligned(const char *what, uintptr_t buffer, size_t element)
 }
 
 // ------------------------------------------------------------------ device side ----
-template <int N>
-struct FloatPack {
-    float v[N];
-};
-
-template <typename T>
-__device__ inline float to_float(T x)
-{
-    return (float)x;
-}
 template <typename T>
 __device__ inline T from_float(float x)
 {

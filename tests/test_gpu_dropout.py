@@ -92,8 +92,8 @@ def test_a_buffer_that_is_too_short_is_refused():
 
 
 def test_known_counters():
-    """Philox4x32-10's published test vectors: counter and key all zeros, and counter and key all ones bits (the first needs
-    block 0, site 0, step 0 and seeds 0; its words' halves decide elements 0 to 7)."""
+    """Philox4x32-10's published test vector for a counter and a key of zeros: block 0, site 0, step 0 and seeds 0; its words'
+    halves decide elements 0 to 7."""
     words = (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)
     bits = [h for w in words for h in (w & 0xFFFF, w >> 16)]
     with Buffers() as b:
