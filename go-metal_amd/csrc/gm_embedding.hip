@@ -13,7 +13,8 @@ namespace gm {
 constexpr int kLookupBlock = 256;
 
 // One lane moves eight elements (16 bytes of a 16-bit type); lanes run over the rows' vectors without gaps, so short
-// rows share a workgroup.  A token outside the vocabulary is padding and gives a row of zeros.
+// rows share a workgroup.  Memory bounds it: 8192 rows of 4096 bf16, dropped out, 23 us = 5.9 TB/s of reads and writes, some
+// rows from the caches.  A single row is one launch's latency, 2.5 us on the device.  A token outside the vocabulary is padding and gives a row of zeros.
 template <typename T>
 __global__ void __launch_bounds__(kLookupBlock)
 lookup_kernel(const T *table, const int *tokens, T *out, uint32_t rows, uint32_t vocab, uint32_t dim, uint32_t per_row,
@@ -43,9 +44,13 @@ lookup_kernel(const T *table, const int *tokens, T *out, uint32_t rows, uint32_t
 // ---------------------------------------------------------------------------------------- sorting the tokens ----
 // A list of up to kSortChunk tokens is sorted by counting: a token's place is the number of tokens before it in the
 // order (token, position).  That is n^2 comparisons without a single dependent pass: 8192 tokens are 67M
-// comparisons over the whole chip.  Longer lists are sorted in chunks; a token's place in the whole is then its
-// place in its chunk plus a binary search in every other one.
-constexpr int kSortChunk = 8192;
+// comparisons over the whole chip, 9.7 us; the vector units' issue bounds it.  Longer lists are sorted in chunks; a
+// token's place in the whole is then its place in its chunk plus a binary search in every other one.  Comparisons grow with
+// the chunk and searches with the number of chunks: 32768 tokens take 27 + 10 us in chunks of 8192 and 9.5 + 11 us in
+// chunks of 2048, so those are taken as long as a token's searches are no more than two a lane of the merge.
+constexpr int kSortChunk = 8192, kShortChunk = 2048;
+constexpr int kMergeLanes = 16;      // lanes that share an element's searches
+constexpr int kShortChunks = 2 * kMergeLanes * kShortChunk;      // the longest list in short chunks
 constexpr int kMostTokens = 1 << 22;      // the merge's searches grow with the square of the list: 512 chunks are enough of them
 constexpr int kSortLanes = 16;        // lanes that share a part of the chunk; each compares kSortOwn tokens of its own with it
 constexpr int kSortOwn = 2;
@@ -55,15 +60,15 @@ constexpr uint32_t kNoToken = 0xFFFFFFFFu;
 constexpr uint32_t kShortVocab = (1u << 19) - 1;
 
 // SHORT: a key is token << 13 | position in the chunk; otherwise the token, and positions are compared where tokens are equal.
-template <bool SHORT>
+template <bool SHORT, int CHUNK>
 __global__ void __launch_bounds__(kSortBlock)
 sort_chunk_kernel(const int *tokens, uint32_t n, uint32_t vocab, int padding, uint32_t *keys, uint32_t *positions)
 {
-    __shared__ __attribute__((aligned(16))) uint32_t all[kSortChunk];
+    __shared__ __attribute__((aligned(16))) uint32_t all[CHUNK];
     __shared__ uint32_t before[kSortRows];
-    constexpr uint32_t kBlocks = kSortChunk / kSortRows;      // per chunk
-    const uint32_t chunk = blockIdx.x / kBlocks, first = chunk * kSortChunk, row = (blockIdx.x - chunk * kBlocks) * kSortRows;
-    const uint32_t len = n - first < kSortChunk ? n - first : kSortChunk;
+    constexpr uint32_t kBlocks = CHUNK / kSortRows;      // per chunk
+    const uint32_t chunk = blockIdx.x / kBlocks, first = chunk * CHUNK, row = (blockIdx.x - chunk * kBlocks) * kSortRows;
+    const uint32_t len = n - first < CHUNK ? n - first : CHUNK;
     if (row >= len) return;
     const uint32_t filled = (len + 4 * kSortSlices - 1) / (4 * kSortSlices) * (4 * kSortSlices);      // whole rounds of fours
     // Padding and tokens outside the vocabulary sort behind everything else; what fills the last round, behind them.
@@ -115,27 +120,34 @@ __device__ inline uint32_t keys_before(const uint32_t *keys, uint32_t n, uint32_
     return lo;
 }
 
+// Sixteen lanes an element, a chunk each at a time: a search's loads depend on each other, the lanes' do not.  11 us for 32768
+// tokens, the latency of eleven loads behind one another.
 __global__ void __launch_bounds__(256)
-merge_chunks_kernel(const uint32_t *keys, const uint32_t *positions, uint32_t n, uint32_t *out_keys, uint32_t *out_positions)
+merge_chunks_kernel(const uint32_t *keys, const uint32_t *positions, uint32_t n, uint32_t chunk, uint32_t *out_keys, uint32_t *out_positions)
 {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t i = blockIdx.x * (256 / kMergeLanes) + threadIdx.x / kMergeLanes, lane = threadIdx.x % kMergeLanes;
     if (i >= n) return;
-    const uint32_t key = keys[i], mine = i / kSortChunk;
-    uint32_t place = i % kSortChunk;
-    for (uint32_t c = 0; c * kSortChunk < n; c++) {
+    const uint32_t key = keys[i], mine = i / chunk;
+    uint32_t place = lane == 0 ? i - mine * chunk : 0;
+    for (uint32_t c = lane; c * chunk < n; c += kMergeLanes) {
         if (c == mine) continue;
-        const uint32_t first = c * kSortChunk, len = n - first < kSortChunk ? n - first : kSortChunk;
+        const uint32_t first = c * chunk, len = n - first < chunk ? n - first : chunk;
         place += keys_before(keys + first, len, key, c < mine);      // equal tokens of earlier chunks come first
     }
-    out_keys[place] = key;
-    out_positions[place] = positions[i];
+#pragma unroll
+    for (int o = kMergeLanes / 2; o; o >>= 1) place += __shfl_xor(place, o);
+    if (lane == 0) {
+        out_keys[place] = key;
+        out_positions[place] = positions[i];
+    }
 }
 
 // ------------------------------------------------------------------------------------------ summing the runs ----
 // The sorted list is cut into pieces of 8 to 32 entries, so that a token that fills a tenth of a batch is summed by
 // many workgroups.  A run that lies in one piece goes straight to its row; of one that crosses a border every piece
 // leaves a partial sum (slot 0: the run the piece begins in the middle of; slot 1: the run it ends in the middle
-// of), which join_runs_kernel adds up in the pieces' order.
+// of), which join_runs_kernel adds up in the pieces' order.  Memory bounds the sums and the fill beside them: 131072 x 2048
+// fp32 from 32768 rows of bf16, 1.21 GB, 220 us = 5.5 TB/s; the joins take 6 to 10 us, latency.
 constexpr int kSumBlock = 64;              // one wavefront, eight elements a lane
 
 // Long pieces leave fewer partial sums, short ones more wavefronts: the longest that leave four for each SIMD.
@@ -456,16 +468,20 @@ try {
     uint32_t *keys = reinterpret_cast<uint32_t *>(workspace + space.keys);
     uint32_t *positions = reinterpret_cast<uint32_t *>(workspace + space.positions);
     const bool chunks = n > kSortChunk;
+    const uint32_t chunk = chunks && n <= kShortChunks ? kShortChunk : kSortChunk;
     uint32_t *to_keys = chunks ? reinterpret_cast<uint32_t *>(workspace + space.chunk_keys) : keys;
     uint32_t *to_positions = chunks ? reinterpret_cast<uint32_t *>(workspace + space.chunk_positions) : positions;
     if (n > 0) {
         // (of a list shorter than a chunk only the workgroups that have rows to place are launched)
-        const uint32_t grid = chunks ? (n + kSortChunk - 1) / kSortChunk * (kSortChunk / kSortRows) : (n + kSortRows - 1) / kSortRows;
-        const auto sort = (uint32_t)vocab_size < kShortVocab ? sort_chunk_kernel<true> : sort_chunk_kernel<false>;
+        const uint32_t grid = chunks ? (n + chunk - 1) / chunk * (chunk / kSortRows) : (n + kSortRows - 1) / kSortRows;
+        const bool word = (uint32_t)vocab_size < kShortVocab;
+        const auto sort = chunk == kSortChunk ? (word ? sort_chunk_kernel<true, kSortChunk> : sort_chunk_kernel<false, kSortChunk>)
+                                              : (word ? sort_chunk_kernel<true, kShortChunk> : sort_chunk_kernel<false, kShortChunk>);
         sort<<<grid, kSortBlock, 0, stream>>>(reinterpret_cast<const int *>(token_buffer), n, (uint32_t)vocab_size, padding_token, to_keys,
                                               to_positions);
     }
-    if (chunks) merge_chunks_kernel<<<(n + 255) / 256, 256, 0, stream>>>(to_keys, to_positions, n, keys, positions);
+    if (chunks)
+        merge_chunks_kernel<<<(n + 256 / kMergeLanes - 1) / (256 / kMergeLanes), 256, 0, stream>>>(to_keys, to_positions, n, chunk, keys, positions);
     a.keys = keys;
     a.positions = positions;
     a.n = n;

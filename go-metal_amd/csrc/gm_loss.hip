@@ -13,6 +13,10 @@
 //   product_kernel  dX and dW
 // 2 N V D operations each: the product of the logits is made once and not again for the gradients; what it costs is
 // the pass of rows_kernel over the workspace.
+// What bounds them: the matrix cores (at the clock the card's power leaves them) the three products, memory rows_kernel and the packing,
+// and for up to 128 tokens the stream of the weights.  4096 x 131072 x 4096 fp16, one token in ten ignored: logits 3.31,
+// rows 0.39 (1.9 GB, 4.9 TB/s), dX 3.06, dW 3.08 ms, 1.2 to 1.3 PFLOP/s; one bf16 token, 131072 x 4096: logits 182 us, 5.9 TB/s.
+// 513 x 10007 x 1000 fp32: packing 27, logits 60, rows 13, dX 45 + 9 (joining its parts), dW 51 us.
 #include "gm_matrix.hpp"
 
 #include "../../include/gometal_hip.h"

@@ -89,7 +89,7 @@ def test_gradient(t, o, n, vocab, dim, kind):
 
 
 @pytest.mark.parametrize("n, vocab, dim, kind", [(8191, 1000, 16, "padded"), (8192, 40, 24, "plain"), (8193, 2000, 8, "padded"),
-                                                 (20000, 3000, 16, "padded"), (40000, 7, 8, "plain"), (16384, 9, 8, "one word"), (9000, 600_000, 4, "padded"),
+                                                 (20000, 3000, 16, "padded"), (65536, 900, 4, "padded"), (65537, 2000, 8, "padded"), (70000, 600_000, 4, "padded"), (40000, 7, 8, "plain"), (16384, 9, 8, "one word"), (9000, 600_000, 4, "padded"),
                                                  (9000, 524_287, 4, "padded"), (9000, 524_286, 4, "padded"), (300, 600_000, 5, "padded")])
 def test_gradient_of_long_lists(n, vocab, dim, kind):
     """Across the borders of the sort's chunks, and words whose occurrences fill many pieces."""
