@@ -70,15 +70,19 @@ class Buffers:
         self.dev = gpu_device()
         assert self.dev is not None, "libgometal_hip.so or the GPU is missing: these operators have no fallback"
         self.lib, self.device = self.dev.lib, self.dev.handle
-        self.owned = []
+        self.owned, self.spaces = [], []
 
     def __enter__(self):
         return self
 
-    def __exit__(self, *exc):
+    def __exit__(self, kind, *exc):
         self.dev.synchronize()
-        for h, _, _ in self.owned:
-            self.dev.free(h)
+        try:
+            for at in self.spaces if kind is None else ():
+                assert np.all(self.dev.to_numpy(at, self.BORDER, np.uint8) == 0xFF), "written outside the workspace"
+        finally:
+            for h, _, _ in self.owned:
+                self.dev.free(h)
 
     def put(self, array, shift=0, stride=None):
         """The array's handle: its rows `stride` elements apart, its start `shift` bytes behind a 256-byte boundary."""
@@ -122,6 +126,7 @@ class Buffers:
         h = self.dev.from_numpy(raw)
         self.owned.append((h, raw.size, (0, raw.size)))
         assert h % align == 0
+        self.spaces += [h, h + self.BORDER + nbytes]
         return h + self.BORDER
 
     def check(self, rc):

@@ -248,6 +248,20 @@ def test_overflow_is_inf_and_nan_spreads_as_in_the_formula():
         assert np.isnan(to_float(got["dx"], F16)[3]).all() and not np.isnan(np.delete(to_float(got["dx"], F16), 3, 0)).any()
 
 
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_row_of_fp32_that_is_not_finite(bad):
+    """It has no power of two; its own loss and slopes are NaN, and what other tokens give is what it was, bit for bit."""
+    n, v, d = 30, 200, 96
+    x, w, targets = data(F32, n, v, d, ignored=0.0)
+    with Buffers() as b:
+        clean = run(b, F32, F32, x, w, targets)
+        x[4, 7] = bad
+        got = run(b, F32, F32, x, w, targets)
+        assert np.isnan(got["losses"][4]) and np.isnan(got["dx"][4]).all() and np.isnan(got["loss"][0])
+        for name in ("losses", "dx"):
+            assert np.array_equal(np.delete(got[name], 4, 0).view(np.uint8), np.delete(clean[name], 4, 0).view(np.uint8)), name
+
+
 @pytest.mark.parametrize("t, o", PAIRS)
 def test_results_repeat(t, o):
     x, w, targets = data(t, 400, 3001, 320)
