@@ -4,7 +4,7 @@
 
 and back: d h1 and d table from the loss, d h0 = d h1 + dropout(d h1), d table += the lookup's gradient of d h0; then the
 mixed-precision step.  Gradients against the formula in 64 bits and against differences of the loss; the step against the CPU
-checker; the whole on a caller's stream, captured into a graph and replayed."""
+oracle; the whole on a caller's stream, captured into a graph and replayed."""
 import ctypes
 
 import numpy as np
@@ -132,9 +132,9 @@ def test_gradient_against_the_formula_and_differences():
         assert abs((losses[0] - losses[1]) / (2 * step) - np.linalg.norm(g)) <= step * step / 6 * third + noise + (want["off"] * np.abs(direction)).sum()
 
 
-def test_steps_follow_the_checker():
+def test_steps_follow_the_oracle():
     """fp16: three mixed-precision steps on the table, the second overflowing.  The gradient that the operators leave is what the
-    checker is given; weights, copy, moments, scale and counters come out bit for bit."""
+    oracle is given; weights, copy, moments, scale and counters come out bit for bit."""
     n, v, d = 200, 300, 72
     table, tokens, targets = data(F16, n, v, d, 6)
     from __graft_entry__ import load_package
