@@ -23,7 +23,7 @@ void clear_error();
 // reference returns from its own @catch block.
 void note_exception() noexcept;
 
-// true when the HIP call succeeded; otherwise records "what: <hip error>".
+// true when the HIP call succeeded; otherwise records "what: <hip error>" and takes the error off the thread.
 bool hip_ok(hipError_t e, const char *what);
 
 struct MultiTensorPlan;

@@ -20,7 +20,8 @@ enum : int {
     kRcType = -19,
 };
 
-// The context's GPU for the length of a call; the caller's current device comes back afterwards.
+// The context's GPU for the length of a call; the caller's current device comes back afterwards.  An error that some
+// earlier HIP call left on the thread is dropped: what hipGetLastError() says behind the launches is about them alone.
 class DeviceScope {
   public:
     explicit DeviceScope(Context *ctx)
@@ -28,6 +29,7 @@ class DeviceScope {
         if (!hip_ok(hipGetDevice(&before_), "hipGetDevice")) return;
         ok_ = before_ == ctx->device_id || make_current(ctx);
         changed_ = ok_ && before_ != ctx->device_id;
+        (void)hipGetLastError();
     }
     ~DeviceScope()
     {

@@ -42,6 +42,7 @@ bool hip_ok(hipError_t e, const char *what)
 {
     if (e == hipSuccess) return true;
     set_error("%s: %s", what, hipGetErrorString(e));
+    (void)hipGetLastError();     // reported here: the thread's next launch must not report it again
     return false;
 }
 
