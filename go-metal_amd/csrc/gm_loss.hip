@@ -834,14 +834,17 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     return s;
 }
 
-// The largest chunk whose plan fits the workspace; bytes of the smallest possible one otherwise.
+// The plan with the most tokens at a time that fits the workspace; otherwise the one that needs the fewest bytes.  (That need not be the
+// one with the fewest tokens: in 16 bits a weight gradient of several chunks takes fp32 sums of its size.)
 static bool fitting_plan(LossPlan &s, size_t bytes, int n, int vocab, int dim, bool weights_fit, int data_type, int gradient_type,
                          bool gradients)
 {
-    s = loss_plan(n, vocab, dim, weights_fit, data_type, gradient_type, gradients, 0);
-    while (s.bytes > bytes && s.chunk > kLeastChunk) {
-        const int half = (s.chunk / 2 + kLeastChunk - 1) / kLeastChunk * kLeastChunk;
-        s = loss_plan(n, vocab, dim, weights_fit, data_type, gradient_type, gradients, half < s.chunk ? half : kLeastChunk);
+    LossPlan next = loss_plan(n, vocab, dim, weights_fit, data_type, gradient_type, gradients, 0);
+    s = next;
+    while (next.bytes > bytes && next.chunk > kLeastChunk) {
+        const int half = (next.chunk / 2 + kLeastChunk - 1) / kLeastChunk * kLeastChunk;
+        next = loss_plan(n, vocab, dim, weights_fit, data_type, gradient_type, gradients, half < next.chunk ? half : kLeastChunk);
+        if (next.bytes <= bytes || next.bytes < s.bytes) s = next;
     }
     return s.bytes <= bytes;
 }

@@ -474,7 +474,7 @@ int execute_embedding_gradient(uintptr_t device, uintptr_t command_queue, uintpt
  * products down to 2^-22 of the largest: about the accuracy of fp32 sums; an element below 2^-18 of its row's largest keeps
  * fewer bits (its error stays below 2^-40 of the row's largest, and the slope's below 2^-39).
  * workspace: gm_linear_cross_entropy_workspace bytes are enough for the fastest form; anything from
- * gm_linear_cross_entropy_least_workspace on works, with fewer tokens at a time.  Aligned to 256.  Both take the weight's
+ * gm_linear_cross_entropy_least_workspace on works, with fewer tokens at a time where that saves memory.  Aligned to 256.  Both take the weight's
  * handle and stride because rows that the kernels can take as they lie (16-bit, dim a multiple of 64, stride of 8, base
  * of 16 bytes) need no copy; handle 0 is the size that always does.  0: sizes that are not offered (more than 2^24 tokens, 2^22
  * words, or a dim above 2^20).
