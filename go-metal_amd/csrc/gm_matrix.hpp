@@ -98,10 +98,9 @@ struct Tile {
     // The wavefront's i-th load of a step.  `base`: the tile's first k of row 0.
     __device__ static inline void load(const char *base, uint32_t offset, uint32_t lds, int wave, int i)
     {
-        // (m0 takes the wavefront's LDS address; one wait state lies between its write and its use)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + (i * WAVES + wave) * 1024), "v"(offset),
-                     "s"(base)
-                     : "memory");
+        // (m0 takes the wavefront's LDS address, as an operand that the compiler writes there; one wait state lies between its
+        // write and its use)
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds + (i * WAVES + wave) * 1024), "v"(offset), "s"(base) : "memory");
     }
 
     // Where this lane reads the fragments of the wavefront's rows row .. row + 16 N - 1: lane l has row l % 16 and k 8 (l / 16)
