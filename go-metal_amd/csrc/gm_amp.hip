@@ -376,7 +376,6 @@ extern "C" {
 
 // ---------------------------------------------------------- mixed precision --
 struct AmpState {
-    uint64_t magic;
     Context *ctx;
     AmpDeviceBlock *d_block;
     int slot;                            // which record of d_block the next step reads (the state as of now)
@@ -389,13 +388,10 @@ struct AmpState {
     int max_in_flight;                   // deepest run-ahead seen (diagnostics)
     unsigned long long last_stamp;       // stamp of the newest step issued (either form); never 0, never repeats
 };
-static const uint64_t kAmpMagic = 0x676D5F616D705F73ull;   // "gm_amp_s"
 
 static AmpState *amp_from_handle(uintptr_t h)
 {
-    if (h == 0) return nullptr;
-    auto *s = reinterpret_cast<AmpState *>(h);
-    return s->magic == kAmpMagic ? s : nullptr;
+    return handle_live(h, HandleKind::kAmpState) ? reinterpret_cast<AmpState *>(h) : nullptr;
 }
 
 static bool amp_upload(AmpState *s)
@@ -511,7 +507,6 @@ static void amp_free(AmpState *s)
 {
     if (s->d_block) (void)hipFree(s->d_block);
     if (s->h_pinned) (void)hipHostFree(s->h_pinned);
-    s->magic = 0;
     delete s;
 }
 
@@ -533,7 +528,6 @@ try {
     Context *ctx = resolve_device(device);
     if (!ctx || !make_current(ctx)) return 0;
     auto *s = new AmpState{};
-    s->magic = kAmpMagic;
     s->ctx = ctx;
     bool ok = hip_ok(hipMalloc(&s->d_block, sizeof(AmpDeviceBlock)), "hipMalloc(amp state)") &&
               hip_ok(hipMemsetAsync(s->d_block, 0, sizeof(AmpDeviceBlock), ctx->stream), "hipMemsetAsync(amp state)") &&
@@ -554,6 +548,7 @@ try {
         amp_free(s);
         return 0;
     }
+    handle_add(s, HandleKind::kAmpState);
     return reinterpret_cast<uintptr_t>(s);
 } catch (...) {
     note_exception();
@@ -563,7 +558,7 @@ try {
 void gm_amp_state_destroy(uintptr_t amp_state)
 try {
     AmpState *s = amp_from_handle(amp_state);
-    if (!s) return;
+    if (!s || !handle_remove(amp_state, HandleKind::kAmpState)) return;
     make_current(s->ctx);
     (void)hipStreamSynchronize(s->ctx->stream);     // ring copies may still be in flight
     amp_free(s);
@@ -595,9 +590,12 @@ try {
 }
 
 int gm_amp_state_max_in_flight(uintptr_t amp_state)
-{
+try {
     AmpState *s = amp_from_handle(amp_state);
     return s ? s->max_in_flight : -16;
+} catch (...) {
+    note_exception();
+    return -6;
 }
 
 int gm_amp_state_set(uintptr_t amp_state, float scale, int growth_tracker)

@@ -90,6 +90,14 @@ uintptr_t registry_remove(uintptr_t buffer);
 // 0 when the handle is not one of ours.
 size_t registry_length(uintptr_t buffer);
 
+// ---- objects of the host that callers hold by their address (queues, loss-scale states) ----
+// Whether a caller's number is one of them is looked up here; what lies at the address is not read to find out.
+enum class HandleKind : int { kQueue, kAmpState };
+void handle_add(const void *object, HandleKind kind);
+bool handle_live(uintptr_t handle, HandleKind kind);
+// false: no such object (any more).
+bool handle_remove(uintptr_t handle, HandleKind kind);
+
 // A freed address may come back with a different length, so whatever was validated against the
 // old allocation must be forgotten: deallocate_metal_buffer calls these (holding ctx->mu) with
 // the freed range.  Only the cached plans that hold a handle inside the range are affected.

@@ -115,6 +115,31 @@ size_t registry_length(uintptr_t buffer)
     return it == g_reg.end() ? 0 : it->second.bytes;
 }
 
+static std::mutex g_handle_mu;
+static std::unordered_map<uintptr_t, HandleKind> g_handles;
+
+void handle_add(const void *object, HandleKind kind)
+{
+    std::lock_guard<std::mutex> lk(g_handle_mu);
+    g_handles[reinterpret_cast<uintptr_t>(object)] = kind;
+}
+
+bool handle_live(uintptr_t handle, HandleKind kind)
+{
+    std::lock_guard<std::mutex> lk(g_handle_mu);
+    const auto it = g_handles.find(handle);
+    return it != g_handles.end() && it->second == kind;
+}
+
+bool handle_remove(uintptr_t handle, HandleKind kind)
+{
+    std::lock_guard<std::mutex> lk(g_handle_mu);
+    const auto it = g_handles.find(handle);
+    if (it == g_handles.end() || it->second != kind) return false;
+    g_handles.erase(it);
+    return true;
+}
+
 // --------------------------------------------------------------- kernels ----
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
@@ -403,18 +428,23 @@ void destroy_metal_device(uintptr_t device)
 }
 
 struct CommandQueue {
-    uint64_t magic;
     Context *ctx;
     hipStream_t stream;      // the context's, or the caller's (gm_command_queue_for_stream)
 };
-static const uint64_t kQueueMagic = 0x676D5F7175657565ull;   // "gm_queue"
+
+static uintptr_t new_queue(Context *ctx, hipStream_t stream)
+{
+    std::unique_ptr<CommandQueue> q(new CommandQueue{ctx, stream});
+    handle_add(q.get(), HandleKind::kQueue);
+    return reinterpret_cast<uintptr_t>(q.release());
+}
 
 uintptr_t create_command_queue(uintptr_t device)
 try {
     if (device == 0) return 0;
     Context *ctx = resolve_device(device);
     if (!ctx) return 0;
-    return reinterpret_cast<uintptr_t>(new CommandQueue{kQueueMagic, ctx, ctx->stream});
+    return new_queue(ctx, ctx->stream);
 } catch (...) {
     note_exception();
     return 0;
@@ -426,19 +456,17 @@ try {
     if (device == 0) return 0;
     Context *ctx = resolve_device(device);
     if (!ctx) return 0;
-    return reinterpret_cast<uintptr_t>(new CommandQueue{kQueueMagic, ctx, reinterpret_cast<hipStream_t>(hip_stream)});
+    return new_queue(ctx, reinterpret_cast<hipStream_t>(hip_stream));
 } catch (...) {
     note_exception();
     return 0;
 }
 
 void release_command_queue(uintptr_t command_queue)
-{
-    if (command_queue == 0) return;
-    auto *q = reinterpret_cast<CommandQueue *>(command_queue);
-    if (q->magic != kQueueMagic) return;
-    q->magic = 0;
-    delete q;
+try {
+    if (handle_remove(command_queue, HandleKind::kQueue)) delete reinterpret_cast<CommandQueue *>(command_queue);
+} catch (...) {
+    note_exception();
 }
 
 uintptr_t allocate_metal_buffer(uintptr_t device, int size, int device_type)
@@ -842,7 +870,7 @@ bool gm::queue_stream(Context *ctx, uintptr_t command_queue, hipStream_t *stream
     *stream = ctx->stream;
     if (command_queue == 0) return true;
     const auto *q = reinterpret_cast<const CommandQueue *>(command_queue);
-    if (q->magic != kQueueMagic || q->ctx != ctx) {
+    if (!handle_live(command_queue, HandleKind::kQueue) || q->ctx != ctx) {
         set_error("the command queue is not one of this device's");
         return false;
     }
