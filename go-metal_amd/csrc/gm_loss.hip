@@ -581,18 +581,24 @@ __device__ inline void finish_as(const ProductArgs &a, O *out, int64_t row, int 
     store8(at, whole, count, v);
 }
 
-// What the sums are multiplied by.
-__device__ inline float output_factor(const ProductArgs &a)
+// What the sums are multiplied by: a factor, then a power of two, apart: small rows' power by itself may lie below the least
+// fp32 number where the output does not.
+struct Factor {
+    float by;
+    int power;
+    __device__ inline float operator()(float v) const { return ldexpf(v * by, power); }
+};
+
+__device__ inline Factor output_factor(const ProductArgs &a)
 {
-    const float by = a.head->coefficient * a.unscale;
-    return a.exponent ? ldexpf(by, *a.exponent - kRowBits - kSlopeBits) : by;
+    return Factor{a.head->coefficient * a.unscale, a.exponent ? *a.exponent - kRowBits - kSlopeBits : 0};
 }
 
 // Eight outputs of one row: times c, added to what is there, rounded once.
-__device__ inline void finish(const ProductArgs &a, float by, int q, int p, float (&v)[8])
+__device__ inline void finish(const ProductArgs &a, const Factor &by, int q, int p, float (&v)[8])
 {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = v[e] * by;
+    for (int e = 0; e < 8; e++) v[e] = by(v[e]);
     if (a.add) {
         const int count = a.p.rows - p < 8 ? a.p.rows - p : 8;
         float more[8];
@@ -609,7 +615,7 @@ __device__ inline void finish(const ProductArgs &a, float by, int q, int p, floa
 // The wavefront's outputs, all of which exist, to rows that begin at multiples of 16 bytes: nothing is left of finish() but
 // the product and the rounding.  (With its cases the stores of a tile took more time than 128 tokens' matrix work.)
 template <typename S, typename O>
-__device__ inline void store_whole(O *out, int64_t stride, float by, uint32_t turn, const f32x4 (&acc)[S::MP][S::MQ])
+__device__ inline void store_whole(O *out, int64_t stride, const Factor &by, uint32_t turn, const f32x4 (&acc)[S::MP][S::MQ])
 {
     const int lane = threadIdx.x & 63;
     constexpr int kLanes = 64 / kTurnRows<S>;
@@ -621,7 +627,7 @@ __device__ inline void store_whole(O *out, int64_t stride, float by, uint32_t tu
         for (int i = 0; i < S::MP; i++) v[i] = acc[i][j];
         turn_rows<S>(turn, v, [&](int, int, float (&o)[8]) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = o[e] * by;
+            for (int e = 0; e < 8; e++) o[e] = by(o[e]);
             store8(at, true, 8, o);
             at += kTurnRows<S> * stride;
         });
@@ -630,13 +636,13 @@ __device__ inline void store_whole(O *out, int64_t stride, float by, uint32_t tu
 
 // The tile at (p0, q0) out of the workgroup's accumulators.
 template <typename S>
-__device__ inline void store_tile(const ProductArgs &a, float by, int p0, int q0, uint32_t split, uint32_t turn, const f32x4 (&acc)[S::MP][S::MQ])
+__device__ inline void store_tile(const ProductArgs &a, const Factor &by, int p0, int q0, uint32_t split, uint32_t turn, const f32x4 (&acc)[S::MP][S::MQ])
 {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave_p = p0 + wave / S::WQ * (S::BP / S::WP), wave_q = q0 + wave % S::WQ * (S::BQ / S::WQ);
     if (wave_p + S::BP / S::WP <= a.p.rows && wave_q + S::BQ / S::WQ <= a.q.rows) {
         if (a.splits > 1 && a.p.rows % 4 == 0) {
-            store_whole<S>(a.partial + ((int64_t)split * a.partial_rows + wave_q) * a.p.rows + wave_p, a.p.rows, 1.0f, turn, acc);
+            store_whole<S>(a.partial + ((int64_t)split * a.partial_rows + wave_q) * a.p.rows + wave_p, a.p.rows, Factor{1.0f, 0}, turn, acc);
             return;
         }
         if (a.splits == 1 && a.out_aligned && !a.accumulate && !a.add && !a.row_of) {
