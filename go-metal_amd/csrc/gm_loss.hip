@@ -130,8 +130,26 @@ __device__ inline void load_padded(const I *row, int c, int dim, bool aligned, f
     load8(row + c, aligned && count == 8, count, v);
 }
 
-// The power of two of a row: its largest element lies below 2^e (0 for a row that is not finite; for a row of zeros less than any
-// other's, so that it takes no part in the largest).  One wavefront; the same in all lanes.
+// The same for a row of an operand.  Of two parts an element that is not finite takes the second, with 0 for the first: of the other
+// operand it then meets the first part alone.  In both, or in the first, it would meet the other's second part as well, whose sign or
+// zero makes NaN of an infinite logit (a word that a bias of -inf bans).
+__device__ inline void split_operand(float (&v)[8], _Float16 *to, int64_t plane, int planes)
+{
+    if (planes != 2) return split_store<_Float16>(v, to, plane, planes);
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        rest[e] = v[e];
+        v[e] = fabsf(v[e]) < INFINITY ? v[e] : 0.0f;
+    }
+    store8(to, true, 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; e++) rest[e] = rest[e] - (float)from_float<_Float16>(v[e]);
+    store8(to + plane, true, 8, rest);
+}
+
+// The power of two of a row: its largest finite element lies below 2^e (for a row without one but zero less than any other's, so that
+// it takes no part in the largest).  One wavefront; the same in all lanes.
 template <typename I>
 __device__ inline int row_exponent(const I *row, int dim, bool aligned)
 {
@@ -143,7 +161,7 @@ __device__ inline int row_exponent(const I *row, int dim, bool aligned)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const uint32_t bits = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-            top = top > bits ? top : bits;
+            top = bits < 0x7F800000u && bits > top ? bits : top;
         }
     }
 #pragma unroll
@@ -153,7 +171,7 @@ __device__ inline int row_exponent(const I *row, int dim, bool aligned)
     }
     if (top == 0) return -200;
     int e = 0;
-    if (top < 0x7F800000u) (void)frexpf(__uint_as_float(top), &e);
+    (void)frexpf(__uint_as_float(top), &e);
     return e;
 }
 
@@ -246,7 +264,7 @@ pack_tokens_kernel(PackArgs a, const I *x, LossHead *head, const int *place_of, 
             if (a.plain) store8(packed + place * a.packed_stride + c, true, 8, v);
             if (a.scaled_planes) {
                 scale8(v, kRowBits - exponent);
-                split_store<_Float16>(v, a.scaled + place * a.packed_stride + c, a.plane, a.scaled_planes);
+                split_operand(v, a.scaled + place * a.packed_stride + c, a.plane, a.scaled_planes);
             }
         }
         return;
@@ -285,7 +303,7 @@ pack_scaled_weights_kernel(const float *w, int64_t w_stride, bool aligned, int r
         float v[8];
         load_padded(from, c, dim, aligned, v);
         scale8(v, kRowBits - exponent);
-        split_store<_Float16>(v, packed + (int64_t)row * width + c, plane, 2);
+        split_operand(v, packed + (int64_t)row * width + c, plane, 2);
     }
 }
 
