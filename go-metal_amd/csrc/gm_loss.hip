@@ -190,6 +190,7 @@ struct PackArgs {
     int64_t x_stride, packed_stride, plane, dx_stride;      // plane: of the scaled rows
     bool aligned;
     int n, dim, width;
+    int first;              // the launch's first workgroup
     bool plain;             // the rows as they are
     // COUNT: what scan_targets_kernel does otherwise
     const int *targets;
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kPackBlock)
 pack_tokens_kernel(PackArgs a, const I *x, LossHead *head, const int *place_of, T *packed, float *losses, I *dx)
 {
     __shared__ int of_wave[kPackBlock / 64];
-    const int i = blockIdx.x;
+    const int i = a.first + (int)blockIdx.x;
     int place, count;
     if (COUNT) {
         // the counted tokens before i (all of them, for the workgroups behind the last token)
@@ -770,7 +771,13 @@ constexpr int kSkew = 64;
 constexpr int kLeastChunk = 256;
 constexpr size_t kKeptBytes = (size_t)4 << 30;      // of exp(s - m) and dS together, unless one chunk needs more
 
-static int tiles(int shape, int64_t p, int64_t q)
+// A launch can address fewer than 2^32 lanes.  Packing goes in launches of at most so many workgroups; a token of rows_kernel takes 512
+// lanes and a tile of 128 x 128 outputs 256, so a chunk has at most kMostChunk tokens, and none of the products more than
+// kMostOutputs outputs (2^23 such tiles; ragged edges add less than a tenth).
+constexpr int kMostGroups = 1 << 23, kMostChunk = 1 << 22;
+constexpr int64_t kMostOutputs = (int64_t)1 << 37;
+
+static int tiles(int shape, int64_t p, int64_t q)      // (below 2^24 for what the plans ask)
 {
     return (int)(((p + kShapeP[shape] - 1) / kShapeP[shape]) * ((q + kShapeQ[shape] - 1) / kShapeQ[shape]));
 }
@@ -806,7 +813,9 @@ static LossPlan loss_plan(int n, int vocab, int dim, bool weights_fit, int data_
     s.pack_weights = data_type == kFloat32 || !weights_fit;
     const size_t entry = s.keep == kKeepNothing ? 0 : s.keep == kKeepHalf ? 2 : 4 + 2 * (s.slope_planes + s.dw_slope_planes);
     if (chunk <= 0) {
-        size_t most = entry ? kKeptBytes / (entry * s.slope_stride) / kLeastChunk * kLeastChunk : (size_t)n;
+        size_t most = kMostOutputs / (vocab > dim ? vocab : dim) / kLeastChunk * kLeastChunk;
+        if (most > kMostChunk) most = kMostChunk;
+        if (entry && most > kKeptBytes / (entry * s.slope_stride)) most = kKeptBytes / (entry * s.slope_stride) / kLeastChunk * kLeastChunk;
         if (most < kLeastChunk) most = kLeastChunk;
         chunk = most < (size_t)n ? (int)most : n;
     }
@@ -932,7 +941,7 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     short *x_exponents = reinterpret_cast<short *>(space + s.x_exponents), *w_exponents = reinterpret_cast<short *>(space + s.w_exponents);
     constexpr bool kFull = std::is_same<I, float>::value;      // fp32: every operand has scales
     const int *targets = reinterpret_cast<const int *>(c.targets);
-    const PackArgs pack{c.hidden_stride, s.x_stride, x_plane, c.dx_stride, c.hidden % 16 == 0 && c.hidden_stride * sizeof(I) % 16 == 0, s.n, s.dim, s.width,
+    PackArgs pack{c.hidden_stride, s.x_stride, x_plane, c.dx_stride, c.hidden % 16 == 0 && c.hidden_stride * sizeof(I) % 16 == 0, s.n, s.dim, s.width, 0,
                         s.plain, targets, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, row_of, row_target, s.scaled_planes, scaled_x,
                         x_exponents};
     const I *hidden = reinterpret_cast<const I *>(c.hidden);
@@ -942,7 +951,10 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
     } else {
         scan_targets_kernel<<<1, kScanBlock, 0, stream>>>(targets, s.n, s.vocab, c.ignore, c.mean, c.gradient_scale, c.amp, head, row_of,
                                                           place_of, row_target);
-        pack_tokens_kernel<I, T, false><<<s.n + kStepK, kPackBlock, 0, stream>>>(pack, hidden, head, place_of, x, losses, dx);
+        for (; pack.first < s.n + kStepK; pack.first += kMostGroups) {
+            const int left = s.n + kStepK - pack.first;
+            pack_tokens_kernel<I, T, false><<<left < kMostGroups ? left : kMostGroups, kPackBlock, 0, stream>>>(pack, hidden, head, place_of, x, losses, dx);
+        }
     }
     Operand w{reinterpret_cast<const short *>(c.weight), c.weight_stride, 0, s.vocab};
     const bool w_aligned = c.weight % 16 == 0 && c.weight_stride * sizeof(I) % 16 == 0;
@@ -951,9 +963,14 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
             reinterpret_cast<const float *>(c.weight), c.weight_stride, w_aligned, s.vocab, s.dim, s.width,
             reinterpret_cast<_Float16 *>(space + s.w), w_plane, w_exponents);
     } else if (s.pack_weights) {
-        const unsigned grid = (unsigned)(((int64_t)s.vocab * (s.width / 8) + kPackBlock - 1) / kPackBlock);
-        pack_weights_kernel<I, T><<<grid, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight), c.weight_stride, w_aligned, s.vocab, s.dim,
-                                                                   s.width, reinterpret_cast<T *>(space + s.w));
+        const int rows_each = (int)((int64_t)kMostGroups * kPackBlock / (s.width / 8));
+        for (int first = 0; first < s.vocab; first += rows_each) {
+            const int rows = s.vocab - first < rows_each ? s.vocab - first : rows_each;
+            const unsigned grid = (unsigned)(((int64_t)rows * (s.width / 8) + kPackBlock - 1) / kPackBlock);
+            pack_weights_kernel<I, T><<<grid, kPackBlock, 0, stream>>>(reinterpret_cast<const I *>(c.weight) + (int64_t)first * c.weight_stride,
+                                                                       c.weight_stride, w_aligned, rows, s.dim, s.width,
+                                                                       reinterpret_cast<T *>(space + s.w) + (int64_t)first * s.width);
+        }
     }
     if (s.dw_slope_planes) largest_exponents_kernel<<<1, 1024, 0, stream>>>(head, x_exponents, w_exponents, kFull ? s.vocab : 0);
     if (s.pack_weights) w = Operand{reinterpret_cast<const short *>(space + s.w), s.width, w_plane, s.vocab};
@@ -1017,8 +1034,8 @@ static void launch_loss(const LossCall &c, const LossPlan &s, hipStream_t stream
 
 static bool loss_sizes(int n, int vocab, int dim, int data_type, int gradient_type)
 {
-    return n >= 0 && n <= 1 << 24 && vocab > 0 && vocab <= 1 << 22 && dim > 0 && dim <= 1 << 20 && known_type(data_type) &&
-           (gradient_type == kFloat32 || gradient_type == data_type);
+    return n >= 0 && n <= 1 << 24 && vocab > 0 && vocab <= 1 << 22 && dim > 0 && dim <= 1 << 20 && (int64_t)vocab * dim <= kMostOutputs &&
+           known_type(data_type) && (gradient_type == kFloat32 || gradient_type == data_type);
 }
 
 }  // namespace gm

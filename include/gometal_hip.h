@@ -477,7 +477,7 @@ int execute_embedding_gradient(uintptr_t device, uintptr_t command_queue, uintpt
  * gm_linear_cross_entropy_least_workspace on works, with fewer tokens at a time where that saves memory.  Aligned to 256.  Both take the weight's
  * handle and stride because rows that the kernels can take as they lie (16-bit, dim a multiple of 64, stride of 8, base
  * of 16 bytes) need no copy; handle 0 is the size that always does.  0: sizes that are not offered (more than 2^24 tokens, 2^22
- * words, or a dim above 2^20).
+ * words or 2^37 weights, or a dim above 2^20).
  * None of the outputs may overlap an input. */
 uintptr_t gm_linear_cross_entropy_workspace(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer, int weight_stride,
                                             int data_type, int gradient_type, int with_gradients);

@@ -30,3 +30,22 @@ def test_the_figure_that_a_refusal_reports_is_accepted(lib, t, o):  # noqa: F811
         assert loss(lib, size=small - 1, **sizes) == -18 and b": at least %d are needed" % small in lib.gm_last_error(), (n, v, d)
         for size in (small, (small + big) // 2, big):
             assert loss(lib, size=size, **sizes) == -3, (n, v, d, size)
+
+
+def test_sizes_that_are_not_offered(lib):  # noqa: F811
+    ask, least = lib.gm_linear_cross_entropy_workspace, lib.gm_linear_cross_entropy_least_workspace
+    for n, v, d, offered in ((1 << 24, 1 << 22, 1 << 15, True), (1 << 24, 1 << 22, (1 << 15) + 1, False), ((1 << 24) + 1, 10, 8, False),
+                             (1, 1 << 17, 1 << 20, True), (1, (1 << 17) + 1, 1 << 20, False), (1, 10, (1 << 20) + 1, False)):
+        for query in (ask, least):
+            for gradients in (0, 1):
+                assert (query(n, v, d, 0, d, 2, 2, gradients) > 0) == offered, (n, v, d)
+        code = loss(lib, n=n, v=v, d=d, xs=d, ws=d, dxs=d, dws=d, size=1000)
+        assert code == (-18 if offered else -5), (n, v, d)
+
+
+@pytest.mark.parametrize("gradients", [0, 1])
+def test_tokens_that_one_launch_cannot_take_are_taken_in_parts(lib, gradients):  # noqa: F811
+    """What is kept of the logits does not grow with the tokens once they pass what a launch can address."""
+    one, two = (lib.gm_linear_cross_entropy_workspace(n, 32000, 64, A, 64, 4, 4, gradients) for n in (1 << 23, 1 << 24))
+    packed = 2 * 128 + 4 * 4      # bytes of a token's row with its skew, and of the lists
+    assert abs(two - one - (packed << 23)) <= 4096
