@@ -17,7 +17,7 @@ constexpr int kLookupBlock = 256;
 // rows from the caches.  A single row is one launch's latency, 2.5 us on the device.  A token outside the vocabulary is padding and gives a row of zeros.
 template <typename T>
 __global__ void __launch_bounds__(kLookupBlock)
-lookup_kernel(const T *table, const int *tokens, T *out, uint32_t rows, uint32_t vocab, uint32_t dim, uint32_t per_row,
+lookup_kernel(const T *table, const int *tokens, T *out, uint64_t first, uint32_t rows, uint32_t vocab, uint32_t dim, uint32_t per_row,
               int64_t table_stride, int64_t out_stride, float scale, DropoutParams d, bool aligned)
 {
     const uint64_t base = (uint64_t)blockIdx.x * kLookupBlock;
@@ -35,7 +35,7 @@ lookup_kernel(const T *table, const int *tokens, T *out, uint32_t rows, uint32_t
         for (int e = 0; e < 8; e++) v[e] = v[e] * scale;
         if (d.state) {
             const DropoutState st = *d.state;
-            drop8(v, (uint64_t)row * dim + col, d, st);
+            drop8(v, first + (uint64_t)row * dim + col, d, st);      // first: the launch's first element
         }
     }
     store8(out + (int64_t)row * out_stride + col, whole, count, v);
@@ -367,10 +367,15 @@ static void launch_lookup(uintptr_t table, uintptr_t tokens, uintptr_t out, int 
 {
     const bool aligned = (table | out) % 16 == 0 && (size_t)table_stride * sizeof(T) % 16 == 0 && (size_t)out_stride * sizeof(T) % 16 == 0;
     const uint32_t per_row = ((uint32_t)dim + 7) / 8;
-    const uint32_t grid = (uint32_t)(((uint64_t)n * per_row + kLookupBlock - 1) / kLookupBlock);
-    lookup_kernel<T><<<grid, kLookupBlock, 0, stream>>>(reinterpret_cast<const T *>(table), reinterpret_cast<const int *>(tokens),
-                                                        reinterpret_cast<T *>(out), (uint32_t)n, (uint32_t)vocab, (uint32_t)dim,
-                                                        per_row, table_stride, out_stride, scale, d, aligned);
+    // (a launch can address fewer than 2^32 lanes: more vectors than 2^31 go in parts of whole rows)
+    const uint32_t rows_each = (1u << 31) / per_row;
+    for (uint32_t first = 0; first < (uint32_t)n; first += rows_each) {
+        const uint32_t rows = (uint32_t)n - first < rows_each ? (uint32_t)n - first : rows_each;
+        const uint32_t grid = (uint32_t)(((uint64_t)rows * per_row + kLookupBlock - 1) / kLookupBlock);
+        lookup_kernel<T><<<grid, kLookupBlock, 0, stream>>>(reinterpret_cast<const T *>(table), reinterpret_cast<const int *>(tokens) + first,
+                                                            reinterpret_cast<T *>(out) + (int64_t)first * out_stride, (uint64_t)first * (uint32_t)dim, rows,
+                                                            (uint32_t)vocab, (uint32_t)dim, per_row, table_stride, out_stride, scale, d, aligned);
+    }
 }
 
 // What the two entry points check alike.
@@ -412,8 +417,8 @@ try {
         !rows_fit("table", table_buffer, (size_t)vocab_size, (size_t)dim, (size_t)table_stride, element) ||
         !rows_fit("output", output_buffer, (size_t)num_tokens, (size_t)dim, (size_t)output_stride, element))
         return kRcRange;
-    if (((uint64_t)num_tokens * (((uint32_t)dim + 7) / 8) + kLookupBlock - 1) / kLookupBlock > 0x7FFFFFFFull) {
-        set_error("a lookup of %d rows of %d elements needs more workgroups than one launch can address", num_tokens, dim);
+    if ((uint64_t)num_tokens * (((uint32_t)dim + 7) / 8) > 1ull << 39) {
+        set_error("a lookup of %d rows of %d elements: at most 2^39 groups of eight elements", num_tokens, dim);
         return kRcRange;
     }
     Context *ctx = resolve_device(device);

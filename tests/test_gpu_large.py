@@ -87,3 +87,34 @@ def loss_of_many_tokens(t, o, n, v, d, marks, gradients):
 def test_as_many_tokens_as_there_may_be(n, gradients):
     marks = np.unique(np.concatenate([np.arange(40), n - 1 - np.arange(40), *(k * (n >> 4) + np.array([-1, 0, 1]) for k in range(1, 16))]))
     loss_of_many_tokens(F16, F16, n, 16, 8, marks, gradients)
+
+
+def kept_at(first, count, p, state, site):
+    """Dropout's mask of `count` elements from the first-th on (a multiple of eight), and a kept element's factor, in whole numbers."""
+    border = int(np.float64(np.float32(p)) * 65536 + 0.5)
+    keep = np.zeros(count, bool)
+    for at in range(0, count, 8):
+        block = (first + at) // 8
+        c, k = [block & 0xFFFFFFFF, block >> 32, site, state[2]], [state[0], state[1]]
+        for _ in range(10):
+            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+        for e in range(min(8, count - at)):
+            keep[at + e] = (c[e // 2] >> (16 * (e % 2)) & 0xFFFF) >= border
+    return keep, np.float32(65536.0 / (65536 - border))
+
+
+def test_a_lookup_of_more_than_one_launch_can_address():
+    """2^32 vectors and some: 69 GB, in three launches, the generator's blocks past 2^32."""
+    n, d, v, t, state = (1 << 23) + 5, 4096, 3, F16, (11, 22, 33, 0)
+    rng = np.random.default_rng(2)
+    table = rng.normal(size=(v, d)).astype(np.float16)
+    ids = (np.arange(n) % 4).astype(np.int32)      # the last of four is padding
+    with Large() as b:
+        hi, ht, s, out = b.put(ids), b.put(table), b.state(state), b.room(n * d * 2)
+        b.check(b.lib.execute_embedding_lookup(b.device, 0, ht, hi, out, n, v, d, d, d, t, 2.0, 0.25, s, 6))
+        for first in (0, (1 << 22) - 1, 1 << 22, (1 << 23) - 1, 1 << 23, n - 1):
+            keep, by = kept_at(first * d, d, 0.25, state, 6)
+            row = table[ids[first]].astype(np.float32) * np.float32(2) if ids[first] < v else np.zeros(d, np.float32)
+            assert np.array_equal(b.read(out, first, 1, d, t)[0], np.where(keep, row * by, np.float32(0)).astype(np.float16)), first
