@@ -480,8 +480,8 @@ try {
                   (uint32_t)vocab_size, 1};
     fill.rows_each = fill.row_bytes * 64 <= 16384 ? 64 : fill.row_bytes < 16384 ? (uint32_t)(16384 / fill.row_bytes) : 1;
     const uint64_t fills = accumulate ? 0 : ((uint64_t)vocab_size + fill.rows_each - 1) / fill.rows_each;
-    if (pieces * a.col_tiles + fills > 0x7FFFFFFFull) {
-        set_error("a gradient of %d rows of %d elements needs more workgroups than one launch can address", num_tokens, dim);
+    if ((pieces * a.col_tiles + fills) * kSumBlock > 0xFFFFFFFFull) {
+        set_error("a gradient of %d rows of %d elements, vocabulary %d, needs more lanes than one launch can address", num_tokens, dim, vocab_size);
         return kRcRange;
     }
     Context *ctx = resolve_device(device);
