@@ -85,6 +85,7 @@ ABI = {
     "execute_embedding_gradient": (i, [u, u, u, u, u, i, i, i, i, i, i, i, f, i, i, f, u, i, u, u]),
     "gm_linear_cross_entropy_workspace": (u, [i, i, i, u, i, i, i, i]),
     "gm_linear_cross_entropy_least_workspace": (u, [i, i, i, u, i, i, i, i]),
+    "gm_linear_cross_entropy_plan": (i, [i, i, i, u, i, i, i, i, u, ip]),
     "execute_linear_cross_entropy": (i, [u, u, u, u, u, u, u, u, u, i, i, i, i, i, i, i, i, i, i, i, f, u, i, u, u]),
     "gm_timer_start": (i, [u]),
     "gm_timer_stop": (f, [u]),

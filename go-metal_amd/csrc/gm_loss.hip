@@ -1062,6 +1062,21 @@ uintptr_t gm_linear_cross_entropy_least_workspace(int num_tokens, int vocab_size
     return s.bytes;
 }
 
+int gm_linear_cross_entropy_plan(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer, int weight_stride, int data_type,
+                                 int gradient_type, int with_gradients, uintptr_t workspace_bytes, int *plan)
+{
+    if (!plan) return kRcNil;
+    if (!known_type(data_type) || (gradient_type != kFloat32 && gradient_type != data_type)) return kRcType;
+    if (!loss_sizes(num_tokens, vocab_size, dim, data_type, gradient_type) || weight_stride < dim) return kRcRange;
+    LossPlan s;
+    if (!fitting_plan(s, workspace_bytes, num_tokens, vocab_size, dim, weights_fit(weight_buffer, dim, weight_stride, data_type), data_type,
+                      gradient_type, with_gradients != 0))
+        return kRcWorkspace;
+    const int is[7] = {s.chunk, s.logits_shape, s.dx_shape, s.dx_splits, s.dw_shape, s.dw_splits, s.sum_weights};
+    for (int k = 0; k < 7; k++) plan[k] = is[k];
+    return 0;
+}
+
 int execute_linear_cross_entropy(uintptr_t device, uintptr_t command_queue, uintptr_t hidden_buffer, uintptr_t weight_buffer,
                                  uintptr_t target_buffer, uintptr_t losses_buffer, uintptr_t loss_buffer,
                                  uintptr_t hidden_gradient_buffer, uintptr_t weight_gradient_buffer, int num_tokens, int vocab_size,

@@ -491,6 +491,13 @@ int execute_linear_cross_entropy(uintptr_t device, uintptr_t command_queue, uint
                                  float gradient_scale, uintptr_t amp_state, int accumulate, uintptr_t workspace,
                                  uintptr_t workspace_bytes);
 
+/* Diagnostics: how execute_linear_cross_entropy would run with a workspace of that many bytes.  plan takes seven ints: the tokens taken
+ * at a time; for the logits the shape of a workgroup's tile (words x tokens; 0: 256 x 256, 1: 128 x 128, 2: 256 x 128, 3: 128 x 32);
+ * for the hidden gradient and for the weight gradient the shape and the parts that its sums are cut into; and 1 if tokens in parts
+ * are summed in fp32 beside a 16-bit weight gradient.  Nothing is launched.  0; -4 plan is NULL; -5, -18, -19 as in the call. */
+int gm_linear_cross_entropy_plan(int num_tokens, int vocab_size, int dim, uintptr_t weight_buffer, int weight_stride, int data_type,
+                                 int gradient_type, int with_gradients, uintptr_t workspace_bytes, int *plan);
+
 /* Measurement helpers used by the benchmark and the profiles. */
 
 /* Records a start / stop event pair on the device's stream; gm_timer_stop
