@@ -159,7 +159,7 @@ static uint32_t piece_for(size_t n, size_t dim)
 
 struct SumArgs {
     const uint32_t *keys, *positions;
-    uint32_t n, vocab, dim;
+    uint32_t n, dim;
     int64_t dy_stride, out_stride;
     float scale;
     int accumulate;
@@ -510,7 +510,6 @@ try {
     a.keys = keys;
     a.positions = positions;
     a.n = n;
-    a.vocab = (uint32_t)vocab_size;
     a.dim = (uint32_t)dim;
     a.dy_stride = output_gradient_stride;
     a.out_stride = table_gradient_stride;
