@@ -469,8 +469,9 @@ int execute_embedding_gradient(uintptr_t device, uintptr_t command_queue, uintpt
  *               read on the device when the call runs.  Either handle may be 0; both: the loss alone.  A gradient that
  *               overflows its type is +-inf, which the mixed-precision step drops.
  *   accumulate: the weight gradient is added to what its buffer holds.
- * A Float32 gradient's product takes the slope of the softmax in two parts of Float16 (22 bits); a 16-bit one's takes it
- * rounded to that type once.  Float32 tensors are multiplied as two parts of Float16, each row scaled by a power of two, with
+ * A Float32 gradient's product takes the slope of the softmax in two parts of Float16 (22 bits).  A 16-bit one's takes it rounded to
+ * that type (the hidden gradient of 16-bit tensors beside a Float32 weight gradient, too); where the weight gradient has 16 bits, the
+ * exponential it is made of has been rounded to Float16 before, 2^-11 of it at most.  Float32 tensors are multiplied as two parts of Float16, each row scaled by a power of two, with
  * products down to 2^-22 of the largest: about the accuracy of fp32 sums; an element below 2^-18 of its row's largest keeps
  * fewer bits (its error stays below 2^-40 of the row's largest, and the slope's below 2^-39).
  * workspace: gm_linear_cross_entropy_workspace bytes are enough for the fastest form; anything from
